@@ -325,6 +325,73 @@ int iris_hip_gemm_fill_tail(const iris_gemm_problem_t *problems, int n_problems,
 int iris_hip_rms_gated_add(float *d_x, const float *d_y, const float *d_w, const float *d_gate,
                            int rows, int cols, float eps, int gate_tanh);
 
+/* ---- microscaled matrices (no counterpart in the reference) ----
+ * Rows of 8-bit (e4m3) or 4-bit (e2m1: 0 .5 1 1.5 2 3 4 6 and a sign) codes
+ * with one power of two per block of 32 columns (OCP microscaling formats):
+ * element (r, c) stands for code * 2^(s[r * ld_s + c / 32] - 127). Codes are
+ * row-major, ld_q bytes a row, e4m3 one and e2m1 half a byte each (the even
+ * column in the low nibble). Rows are padded to whole 128 columns: padding
+ * codes are 0 and padding blocks' scales 0. Codes and scales start on 16
+ * bytes, ld_q and ld_s are multiples of 16 and at least iris_hip_mx_ld_codes
+ * and iris_hip_mx_ld_scales of the columns (the scale bytes from the padded
+ * columns to the next multiple of 16 are never read for their value). Rows of
+ * a checkpoint in this format are used as they are. */
+enum { IRIS_MX_FP8 = 0, IRIS_MX_FP4 = 1 };
+typedef struct {
+    uint8_t *q, *s;      /* codes, scales */
+    int ld_q, ld_s;      /* bytes per row */
+    int fmt;
+} iris_mx_t;
+int iris_hip_mx_ld_codes(int fmt, int cols);
+int iris_hip_mx_ld_scales(int cols);
+
+/* Rows of x (f32, or bf16 if is_bf16; ldx elements a row, any alignment) to
+ * microscaled rows, padding included; rows behind the last stay as they are.
+ * With e = floor(log2(largest magnitude of a block)) the scale is
+ * 2^max(e - 2, -127) (e2m1) or 2^max(e - 8, -127) (e4m3) and a code
+ * x / scale rounded to the nearest value, ties to even, at most 6 or 448 in
+ * magnitude. A block of zeros has scale byte 0. A block that holds a NaN or
+ * an infinity has scale byte 255, which makes all of it NaN, and codes 0. */
+int iris_hip_mx_quantize(const iris_mx_t *out, const void *d_x, int is_bf16, int ldx, int rows, int cols);
+/* The values of a microscaled matrix, f32 or bf16 (rounded once where a
+ * value has no bf16 of its own, below 2^-126). */
+int iris_hip_mx_dequantize(void *d_y, int is_bf16, int ldy, const iris_mx_t *a, int rows, int cols);
+
+/* RMSNorm with the residual's addition: per row
+ *   t = x + gate * d          (one rounding to f32; gate NULL: 1; d NULL: t = x)
+ *   out = t / sqrt(mean(t^2) + eps) * w (* scale if given), microscaled
+ * t goes to x_out (required with d, not written without it): x itself with its
+ * row stride, or rows that overlap neither x nor d. The statistics are held in 64 bits and the codes
+ * are those of the exact quotient of t's f32 values. x, d, x_out of any
+ * alignment. */
+typedef struct {
+    const float *x; int ldx;
+    const void *d; int ldd; int d_bf16;   /* f32 rows, or bf16 */
+    const float *gate;                    /* [cols] */
+    float *x_out; int ldxo;
+    const float *w, *scale;               /* [cols] */
+    iris_mx_t out;
+    int rows, cols;
+    float eps;
+} iris_mx_norm_t;
+int iris_hip_mx_rmsnorm(const iris_mx_norm_t *a);
+
+/* out = A[M,K] . W[N,K]^T with A either format and W 4-bit, f32 sums and the
+ * epilogues of iris_hip_gemm: F32, BF16, GATED_ADD, ADD with vec as there, and
+ * SWIGLU (N % 64 == 0, no vec) into bf16 rows, or with mx_out.q set into the
+ * microscaled rows mx_out instead (out unused), from the f32 values and with
+ * their padding. Any M, N, K. d_ws (or NULL): f32 workspace that lets products
+ * of few tiles be split over K, summed in a fixed order. Calls that share a
+ * workspace must not overlap. */
+typedef struct {
+    iris_mx_t A, W;
+    void *out;
+    const float *vec;
+    int M, N, K, ldo, epi;
+    iris_mx_t mx_out;
+} iris_mx_gemm_t;
+int iris_hip_mx_gemm(const iris_mx_gemm_t *problem, float *d_ws, size_t ws_bytes);
+
 /* ---- attention pieces ---- */
 /* Per (row, head) RMSNorm of Q and K (x w_q / w_k, rows < split use set A) and
  * rotary embedding from per-row cos/sin tables [rows][128] (pairs 2i, 2i+1).

@@ -1,0 +1,655 @@
+/*
+ * mx.hip - microscaled matrices (4-bit e2m1 and 8-bit e4m3 codes, one power of
+ * two per 32 columns of a row): quantisation, RMSNorm of an updated residual
+ * stream with such an output, and the product with 4-bit weights on the
+ * scaled matrix instructions. No counterpart in the reference, whose linears
+ * are f32 and bf16 (iris_kernels.c:146-336).
+ *
+ * Block scale: with E the biased exponent of the block's largest magnitude,
+ * floor(log2 max) = E - 127, so the scale byte is max(E - emax, 0) for zero,
+ * subnormal and normal values alike, emax the exponent of the largest code (2
+ * or 8). x / scale is exact in f32 wherever the result is not far below the
+ * smallest code.
+ */
+#include "iris_internal.h"
+
+namespace {
+
+constexpr int NT = 256;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+/* 8 f32 values, the 8 columns of a lane; the 4 lanes of a quad hold a block of 32 */
+struct Row8 {
+    float v[8];
+};
+
+__device__ __forceinline__ uint32_t quad_maxu(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));
+    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));
+}
+
+/* scale byte of a block whose largest magnitude has these f32 bits */
+template <int FMT> __device__ __forceinline__ int mx_scale(uint32_t top) {
+    constexpr int EMAX = FMT == IRIS_MX_FP4 ? 2 : 8;
+    return top >= 0x7f800000u ? 255 : max((int)(top >> 23) - EMAX, 0);
+}
+
+/* 1 / scale; 0 for a block that holds a NaN or an infinity */
+__device__ __forceinline__ float mx_inv(int s) { return s == 255 ? 0.0f : __int_as_float((254 - s) << 23); }
+
+/* codes of 4 values, code of v[0] lowest. e2m1 conversion saturates by
+ * itself; e4m3 has a NaN above 448, hence the clamp. */
+__device__ __forceinline__ uint32_t mx_fp8x4(float a, float b, float c, float d, float inv) {
+    auto y = [inv](float v) { return inv == 0.0f ? 0.0f : __builtin_amdgcn_fmed3f(v * inv, -448.0f, 448.0f); };
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(y(a), y(b), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y(c), y(d), r, true);
+}
+__device__ __forceinline__ uint32_t mx_fp4x4(float a, float b, float c, float d, float inv) {
+    auto y = [inv](float v) { return inv == 0.0f ? 0.0f : v * inv; };
+    uint32_t r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y(a), y(b), 1.0f, 0);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y(c), y(d), 1.0f, 1) & 0xffffu;
+}
+
+/* the lane's 8 columns from c (a multiple of 8) on, of one row */
+template <int FMT> __device__ __forceinline__ void mx_put8(uint8_t *q, uint8_t *s, int c, const Row8 &x) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x.v[i]) & 0x7fffffffu);
+    const int sb = mx_scale<FMT>(quad_maxu(top));
+    const float inv = mx_inv(sb);
+    if constexpr (FMT == IRIS_MX_FP8) {
+        *(uint2 *)(q + c) = make_uint2(mx_fp8x4(x.v[0], x.v[1], x.v[2], x.v[3], inv),
+                                       mx_fp8x4(x.v[4], x.v[5], x.v[6], x.v[7], inv));
+    } else {
+        *(uint32_t *)(q + c / 2) = mx_fp4x4(x.v[0], x.v[1], x.v[2], x.v[3], inv) |
+                                   mx_fp4x4(x.v[4], x.v[5], x.v[6], x.v[7], inv) << 16;
+    }
+    if ((threadIdx.x & 3) == 0) s[c / 32] = (uint8_t)sb;
+}
+
+/* 8 columns from c on of a row of f32 or bf16, zeros past cols; vec: 16-byte accesses are allowed */
+template <bool BF16> __device__ __forceinline__ Row8 load8(const void *row, int c, int cols, bool vec) {
+    Row8 x;
+    if (vec && c + 8 <= cols) {
+        if constexpr (BF16) {
+            const u32x4 t = *(const u32x4 *)((const uint16_t *)row + c);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x.v[2 * i] = __uint_as_float(t[i] << 16);
+                x.v[2 * i + 1] = __uint_as_float(t[i] & 0xffff0000u);
+            }
+        } else {
+            const float4 a = *(const float4 *)((const float *)row + c), b = *(const float4 *)((const float *)row + c + 4);
+            x.v[0] = a.x; x.v[1] = a.y; x.v[2] = a.z; x.v[3] = a.w;
+            x.v[4] = b.x; x.v[5] = b.y; x.v[6] = b.z; x.v[7] = b.w;
+        }
+        return x;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if constexpr (BF16) x.v[i] = c + i < cols ? bf2f(((const uint16_t *)row)[c + i]) : 0.0f;
+        else x.v[i] = c + i < cols ? ((const float *)row)[c + i] : 0.0f;
+    }
+    return x;
+}
+
+/* One lane per 8 columns, rows one after the other (cpr = padded columns / 8
+ * lanes each, a multiple of 16, so a quad stays in its block). */
+template <int FMT, bool BF16>
+__global__ __launch_bounds__(NT) void mx_quantize_kernel(uint8_t *q, uint8_t *s, int ld_q, int ld_s, const void *x,
+                                                         int ldx, int cols, uint32_t cpr, uint32_t n, bool vec) {
+    const uint32_t i = blockIdx.x * NT + threadIdx.x;
+    if (i >= n) return;
+    const uint32_t row = i / cpr;
+    const int c = (int)(i - row * cpr) * 8;
+    const void *xr = (const char *)x + (size_t)row * ldx * (BF16 ? 2 : 4);
+    mx_put8<FMT>(q + (size_t)row * ld_q, s + (size_t)row * ld_s, c, load8<BF16>(xr, c, cols, vec));
+}
+
+/* 2^(s - 127); NaN for 255 */
+__device__ __forceinline__ float mx_two(int s) {
+    return s == 255 ? __int_as_float(0x7fc00000) : s ? __int_as_float(s << 23) : __int_as_float(0x00400000);
+}
+
+template <int FMT, bool BF16>
+__global__ __launch_bounds__(NT) void mx_dequantize_kernel(void *y, int ldy, const uint8_t *q, const uint8_t *s,
+                                                           int ld_q, int ld_s, int cols, uint32_t cpr, uint32_t n,
+                                                           bool vec) {
+    const uint32_t i = blockIdx.x * NT + threadIdx.x;
+    if (i >= n) return;
+    const uint32_t row = i / cpr;
+    const int c = (int)(i - row * cpr) * 8;
+    const uint8_t *qr = q + (size_t)row * ld_q;
+    const float two = mx_two(s[(size_t)row * ld_s + c / 32]);
+    float v[8];
+    if constexpr (FMT == IRIS_MX_FP8) {
+        const uint2 t = *(const uint2 *)(qr + c);
+        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)t.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)t.x, true);
+        const f32x2 d = __builtin_amdgcn_cvt_pk_f32_fp8((int)t.y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8((int)t.y, true);
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = d.x; v[5] = d.y; v[6] = e.x; v[7] = e.y;
+    } else {
+        const uint32_t t = *(const uint32_t *)(qr + c / 2);
+        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(t, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(t, 1.0f, 1);
+        const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(t, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(t, 1.0f, 3);
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = d.x; v[5] = d.y; v[6] = e.x; v[7] = e.y;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] *= two;
+    if constexpr (BF16) {
+        uint16_t *yr = (uint16_t *)y + (size_t)row * ldy;
+        u32x4 t;
+#pragma unroll
+        for (int j = 0; j < 4; j++) t[j] = (uint32_t)f2bf_hw(v[2 * j]) | (uint32_t)f2bf_hw(v[2 * j + 1]) << 16;
+        if (vec && c + 8 <= cols) *(u32x4 *)(yr + c) = t;
+        else
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (c + j < cols) yr[c + j] = (uint16_t)(t[j >> 1] >> (16 * (j & 1)));
+    } else {
+        float *yr = (float *)y + (size_t)row * ldy;
+        if (vec && c + 8 <= cols) {
+            *(float4 *)(yr + c) = make_float4(v[0], v[1], v[2], v[3]);
+            *(float4 *)(yr + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (c + j < cols) yr[c + j] = v[j];
+    }
+}
+
+/* ---- RMSNorm of an updated stream ----
+ * t = f32(x + gate d) into x_out; y = t / sqrt(mean t^2 + eps) w (scale),
+ * quantised. Codes are those of the formula in exact arithmetic: the sum of
+ * squares and y are held in 64 bits, and y goes to f32 rounded to odd (toward
+ * zero, last bit set where anything was cut off), which keeps its exponent
+ * and every later rounding to fewer bits as of y itself. So a code depends
+ * neither on the order of the sum nor on an f32 rounding next to a border of
+ * two codes (5e-6 of all elements otherwise). */
+struct NormParams {
+    const float *x, *gate, *w, *scale;
+    const void *d;
+    float *x_out;
+    uint8_t *q, *s;
+    int ldx, ldd, ldxo, ld_q, ld_s, cols, cols_pad;
+    float eps;
+    bool vx, vd, vo;   /* 16-byte accesses to x, d, x_out */
+};
+
+__device__ __forceinline__ float to_odd(double y) {
+    const float h = (float)y;
+    uint32_t u = __float_as_uint(h);
+    if (fabs((double)h) > fabs(y)) u--;         /* toward zero; an infinity becomes the largest number */
+    if ((double)h != y) u |= 1;
+    return isnan(y) ? h : __uint_as_float(u);
+}
+
+template <int DT> __device__ __forceinline__ Row8 norm_row8(const NormParams &P, size_t row, int c, bool store) {
+    Row8 x = load8<false>(P.x + row * P.ldx, c, P.cols, P.vx);
+    if constexpr (DT) {
+        const Row8 d = load8<DT == 2>((const char *)P.d + row * P.ldd * (DT == 2 ? 2 : 4), c, P.cols, P.vd);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x.v[i] = P.gate ? fmaf(c + i < P.cols ? P.gate[c + i] : 0.0f, d.v[i], x.v[i]) : x.v[i] + d.v[i];
+        if (store) {
+            float *o = P.x_out + row * P.ldxo + c;
+            if (P.vo && c + 8 <= P.cols) {
+                *(float4 *)o = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
+                *(float4 *)(o + 4) = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
+            } else
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (c + i < P.cols) o[i] = x.v[i];
+        }
+    }
+    return x;
+}
+
+/* DT: 0 no d, 1 f32, 2 bf16. One block per row, R chunks of 8 columns a
+ * thread held in registers; R 0: any length, the row read twice (the second
+ * time from x_out where there is a d: the thread's own stores). */
+template <int FMT, int DT, int R> __global__ __launch_bounds__(NT) void mx_rmsnorm_kernel(const NormParams P) {
+    __shared__ double red[NT / IRIS_WAVE];
+    const size_t row = blockIdx.x;
+    Row8 t[R ? R : 1];
+    double ss = 0.0;
+    auto square = [&](const Row8 &x) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss = fma((double)x.v[i], (double)x.v[i], ss);
+    };
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int c = (r * NT + (int)threadIdx.x) * 8;
+            if (c < P.cols_pad) {
+                t[r] = norm_row8<DT>(P, row, c, true);
+                square(t[r]);
+            }
+        }
+    } else {
+        for (int c = (int)threadIdx.x * 8; c < P.cols_pad; c += NT * 8) square(norm_row8<DT>(P, row, c, true));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
+    __syncthreads();
+    ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < NT / IRIS_WAVE; i++) ss += red[i];
+    const double inv = 1.0 / sqrt(ss / P.cols + (double)P.eps);
+    auto put = [&](const Row8 &x, int c) {
+        Row8 y;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const bool in = c + i < P.cols;
+            double v = (double)x.v[i] * inv * (double)(in ? P.w[c + i] : 0.0f);
+            if (P.scale) v *= (double)(in ? P.scale[c + i] : 0.0f);
+            y.v[i] = in ? to_odd(v) : 0.0f;
+        }
+        mx_put8<FMT>(P.q + row * P.ld_q, P.s + row * P.ld_s, c, y);
+    };
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int c = (r * NT + (int)threadIdx.x) * 8;
+            if (c < P.cols_pad) put(t[r], c);
+        }
+    } else {
+        NormParams P2 = P;
+        if constexpr (DT != 0) {
+            P2.x = P.x_out;
+            P2.ldx = P.ldxo;
+            P2.vx = P.vo;
+        }
+        for (int c = (int)threadIdx.x * 8; c < P.cols_pad; c += NT * 8) put(norm_row8<0>(P2, row, c, false), c);
+    }
+}
+
+/* ---- product ----
+ * out[m][n] = sum over K of A[m][k] W[n][k] on v_mfma_scale_f32_16x16x128:
+ * W is the first operand, so a lane ends with 4 consecutive n of one m. Lane
+ * l = 16 g + r of an operand holds row r: of e2m1 columns 32 g .. 32 g + 31
+ * (16 bytes), of e4m3 columns 16 g .. 16 g + 15 and 64 + 16 g .. (two times
+ * 16 bytes), and the scale of block g of the row in its byte. */
+struct MxGemm {
+    const uint8_t *aq, *as, *wq, *ws;
+    int lda, ldas, ldw, ldws;
+    void *out;
+    const float *vec;
+    int M, N, steps, ldo, epi;
+    uint8_t *oq, *os;      /* SWIGLU: microscaled output, NULL: bf16 into out */
+    int ldoq, ldos, ofmt;
+};
+
+/* The instruction adds its products in groups of 8 neighbouring columns and
+ * keeps, of a group, bits down to 2^-13 of the largest product's power of two
+ * (measured; between groups and with the accumulator it keeps f32). Products
+ * of two e2m1 codes span 2^6 and lose nothing; those with e4m3 codes span more,
+ * which leaves sums 2e-5 off (512 x 2560 x 9728). So A's e4m3 codes go through
+ * it twice, those of magnitude 2 and more (exponents 1 .. 8) and those below
+ * (lowest bit 2^-9 to 2^0): with W's lowest bit 2^-1 and highest 2^2 either
+ * span is within 13 powers of two, and the sums are f32 sums. */
+template <int AF>
+__device__ __forceinline__ f32x4 mx_mfma(const u32x4 &w, const i32x8 &a, const f32x4 &c, int sw, int sa) {
+    const i32x8 w8 = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, a, c, 4, AF == IRIS_MX_FP8 ? 0 : 4, 0, sw, 0, sa);
+}
+
+/* e4m3 codes of magnitude 2 and more (bit 6 set), and the others */
+__device__ __forceinline__ void mx_split(const i32x8 &a, i32x8 &hi, i32x8 &lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t big = (((uint32_t)a[i] >> 6) & 0x01010101u) * 255u;
+        hi[i] = (int)((uint32_t)a[i] & big);
+        lo[i] = (int)((uint32_t)a[i] & ~big);
+    }
+}
+
+/* one lane's 4 columns n .. n + 3 of row m through the plain epilogues */
+__device__ __forceinline__ void mx_store4(const MxGemm &P, int m, int n, const f32x4 &x, bool aligned) {
+    const float vd = P.epi == IRIS_EPI_GATED_ADD ? 1.0f : 0.0f;
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) v[r] = P.vec && n + r < P.N ? P.vec[n + r] : vd;
+    const size_t o = (size_t)m * P.ldo + n;
+    if (aligned && n + 4 <= P.N) {
+        if (P.epi == IRIS_EPI_BF16) {
+            *(uint2 *)((uint16_t *)P.out + o) =
+                make_uint2((uint32_t)f2bf_hw(x[0] + v[0]) | (uint32_t)f2bf_hw(x[1] + v[1]) << 16,
+                           (uint32_t)f2bf_hw(x[2] + v[2]) | (uint32_t)f2bf_hw(x[3] + v[3]) << 16);
+            return;
+        }
+        float4 *dst = (float4 *)((float *)P.out + o);
+        float4 y = make_float4(x[0] + v[0], x[1] + v[1], x[2] + v[2], x[3] + v[3]);
+        if (P.epi == IRIS_EPI_GATED_ADD) {
+            y = *dst;
+            y.x += v[0] * x[0]; y.y += v[1] * x[1]; y.z += v[2] * x[2]; y.w += v[3] * x[3];
+        } else if (P.epi == IRIS_EPI_ADD) {
+            const float4 t = *dst;
+            y.x += t.x; y.y += t.y; y.z += t.z; y.w += t.w;
+        }
+        *dst = y;
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        if (n + r >= P.N) continue;
+        float *f = (float *)P.out + o + r;
+        if (P.epi == IRIS_EPI_BF16) ((uint16_t *)P.out)[o + r] = f2bf_hw(x[r] + v[r]);
+        else if (P.epi == IRIS_EPI_GATED_ADD) *f += v[r] * x[r];
+        else if (P.epi == IRIS_EPI_ADD) *f = x[r] + v[r] + *f;
+        else *f = x[r] + v[r];
+    }
+}
+
+/* a 64-column gate / up group from n on (gate tiles 0, 1, up tiles 2, 3): 8
+ * values of row m in each of 4 lanes 16 apart, one block of 32 columns of the
+ * output. Whole waves call it: the block's maximum is taken over the lanes. */
+__device__ __forceinline__ void mx_store_swiglu(const MxGemm &P, int m, int n, const f32x4 &g0, const f32x4 &g1,
+                                                const f32x4 &u0, const f32x4 &u1, bool aligned) {
+    const int lg = (threadIdx.x >> 4) & 3, col = n / 2 + 4 * lg;
+    const bool in = m < P.M && n < P.N;   /* N % 64 == 0: the whole group or nothing */
+    float y[8];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        y[r] = g0[r] / (1.0f + expf(-g0[r])) * u0[r];
+        y[4 + r] = g1[r] / (1.0f + expf(-g1[r])) * u1[r];
+    }
+    if (!P.oq) {
+        if (!in) return;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            uint16_t *dst = (uint16_t *)P.out + (size_t)m * P.ldo + col + 16 * h;
+            uint16_t b[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) b[r] = f2bf_hw(y[4 * h + r]);
+            if (aligned)
+                *(uint2 *)dst = make_uint2((uint32_t)b[0] | (uint32_t)b[1] << 16, (uint32_t)b[2] | (uint32_t)b[3] << 16);
+            else
+#pragma unroll
+                for (int r = 0; r < 4; r++) dst[r] = b[r];
+        }
+        return;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    if (!in) return;
+    uint8_t *q = P.oq + (size_t)m * P.ldoq, *s = P.os + (size_t)m * P.ldos;
+    int sb;
+    if (P.ofmt == IRIS_MX_FP8) {
+        sb = mx_scale<IRIS_MX_FP8>(top);
+        const float inv = mx_inv(sb);
+        *(uint32_t *)(q + col) = mx_fp8x4(y[0], y[1], y[2], y[3], inv);
+        *(uint32_t *)(q + col + 16) = mx_fp8x4(y[4], y[5], y[6], y[7], inv);
+    } else {
+        sb = mx_scale<IRIS_MX_FP4>(top);
+        const float inv = mx_inv(sb);
+        *(uint16_t *)(q + col / 2) = (uint16_t)mx_fp4x4(y[0], y[1], y[2], y[3], inv);
+        *(uint16_t *)(q + col / 2 + 8) = (uint16_t)mx_fp4x4(y[4], y[5], y[6], y[7], inv);
+    }
+    if (lg == 0) s[n / 64] = (uint8_t)sb;
+    /* zero blocks up to the padded width, behind the last group */
+    if (n + 64 == P.N)
+        for (int b = P.N / 64; b & 3; b++) {
+            if (P.ofmt == IRIS_MX_FP8) *(uint2 *)(q + 32 * b + 8 * lg) = make_uint2(0, 0);
+            else *(uint32_t *)(q + 16 * b + 4 * lg) = 0;
+            if (lg == 0) s[b] = 0;
+        }
+}
+
+/* A block's 8 waves share 16 FM rows of A and 16 FN of W and take every
+ * eighth K step of 128 each, fragments straight from global memory; their sums
+ * are added in wave order through LDS. */
+template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm_direct_kernel(const MxGemm P) {
+    __shared__ f32x4 part[8][64];
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4, wave = tid >> 6;
+    const int tiles_n = (P.N + 16 * FN - 1) / (16 * FN);
+    const int m0 = (int)(blockIdx.x / tiles_n) * 16 * FM, n0 = (int)(blockIdx.x % tiles_n) * 16 * FN;
+    const uint8_t *ap[FM], *sap[FM], *wp[FN], *swp[FN];
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+        const size_t m = min(m0 + 16 * i + lr, P.M - 1);   /* rows past the end repeat the last; not stored */
+        ap[i] = P.aq + m * P.lda + 16 * lg;
+        sap[i] = P.as + m * P.ldas + lg;
+    }
+#pragma unroll
+    for (int j = 0; j < FN; j++) {
+        const size_t n = min(n0 + 16 * j + lr, P.N - 1);
+        wp[j] = P.wq + n * P.ldw + 16 * lg;
+        swp[j] = P.ws + n * P.ldws + lg;
+    }
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = wave; k < P.steps; k += 8) {
+        u32x4 w[FN];
+        i32x8 a[FM];
+        int sw[FN], sa[FM];
+#pragma unroll
+        for (int j = 0; j < FN; j++) {
+            w[j] = *(const u32x4 *)(wp[j] + (size_t)k * 64);
+            sw[j] = swp[j][k * 4];
+        }
+#pragma unroll
+        for (int i = 0; i < FM; i++) {
+            sa[i] = sap[i][k * 4];
+            if constexpr (AF == IRIS_MX_FP8) {
+                const u32x4 lo = *(const u32x4 *)(ap[i] + (size_t)k * 128), hi = *(const u32x4 *)(ap[i] + (size_t)k * 128 + 64);
+                a[i] = (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+            } else {
+                const u32x4 lo = *(const u32x4 *)(ap[i] + (size_t)k * 64);
+                a[i] = (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < FM; i++) {
+            i32x8 hi = a[i], lo = a[i];
+            if constexpr (AF == IRIS_MX_FP8) mx_split(a[i], hi, lo);
+#pragma unroll
+            for (int j = 0; j < FN; j++) {
+                acc[i][j] = mx_mfma<AF>(w[j], hi, acc[i][j], sw[j], sa[i]);
+                if constexpr (AF == IRIS_MX_FP8) acc[i][j] = mx_mfma<AF>(w[j], lo, acc[i][j], sw[j], sa[i]);
+            }
+        }
+    }
+    /* wave i % 8 sums tile i of a row of tiles */
+    const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
+    f32x4 mine[FM][FN];   /* only wave 0 keeps the sums */
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) {
+            __syncthreads();
+            part[wave][lane] = acc[i][j];
+            __syncthreads();
+            f32x4 s = part[0][lane];
+#pragma unroll
+            for (int w = 1; w < 8; w++) s += part[w][lane];
+            mine[i][j] = s;
+        }
+    if (wave) return;
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+        const int m = m0 + 16 * i + lr;
+        if (FN == 4 && P.epi == IRIS_EPI_SWIGLU) {
+            if constexpr (FN == 4) mx_store_swiglu(P, m, n0, mine[i][0], mine[i][1], mine[i][2], mine[i][3], aligned);
+        } else if (m < P.M) {
+#pragma unroll
+            for (int j = 0; j < FN; j++) mx_store4(P, m, n0 + 16 * j + 4 * lg, mine[i][j], aligned);
+        }
+    }
+}
+
+/* ---- argument checks ---- */
+int pad_to(long long v, int to) { return (int)((v + to - 1) / to * to); }
+
+int check_mx(const char *what, const iris_mx_t &a, int cols) {
+    if (a.fmt != IRIS_MX_FP8 && a.fmt != IRIS_MX_FP4) return iris_set_error("%s: format %d", what, a.fmt);
+    if (!a.q || !a.s) return iris_set_error("%s: null codes or scales", what);
+    if (cols > (1 << 30)) return iris_set_error("%s: %d columns", what, cols);
+    if (((uintptr_t)a.q & 15) || ((uintptr_t)a.s & 15) || (a.ld_q & 15) || (a.ld_s & 15))
+        return iris_set_error("%s: codes and scales need 16-byte aligned rows", what);
+    if (a.ld_q < iris_hip_mx_ld_codes(a.fmt, cols) || a.ld_s < iris_hip_mx_ld_scales(cols))
+        return iris_set_error("%s: row strides %d, %d hold less than %d columns", what, a.ld_q, a.ld_s, cols);
+    return 0;
+}
+
+bool rows16(const void *p, long long ld, int elt) { return ((uintptr_t)p & 15) == 0 && (ld * elt & 15) == 0; }
+
+}  // namespace
+
+extern "C" {
+
+int iris_hip_mx_ld_codes(int fmt, int cols) {
+    return fmt == IRIS_MX_FP4 ? pad_to(cols, 128) / 2 : pad_to(cols, 128);
+}
+int iris_hip_mx_ld_scales(int cols) { return pad_to(cols, 512) / 32; }
+
+/* rows per launch: lanes counted in 32 bits */
+static int rows_per_launch(uint32_t cpr) { return (int)((1u << 30) / cpr); }
+
+int iris_hip_mx_quantize(const iris_mx_t *out, const void *x, int is_bf16, int ldx, int rows, int cols) {
+    if (rows <= 0 || cols <= 0) return 0;
+    if (!out || !x) return iris_set_error("mx_quantize: null argument");
+    if (check_mx("mx_quantize", *out, cols)) return -1;
+    if (ldx < cols) return iris_set_error("mx_quantize: row stride %d of %d columns", ldx, cols);
+    if (!iris_hip_available()) return -1;
+    const int es = is_bf16 ? 2 : 4;
+    const uint32_t cpr = (uint32_t)pad_to(cols, 128) / 8;
+    const bool vec = rows16(x, ldx, es);
+    for (int r0 = 0, nr; r0 < rows; r0 += nr) {
+        nr = rows - r0 < rows_per_launch(cpr) ? rows - r0 : rows_per_launch(cpr);
+        const uint32_t n = (uint32_t)nr * cpr;
+        const dim3 grid((n + NT - 1) / NT);
+        uint8_t *q = out->q + (size_t)r0 * out->ld_q, *s = out->s + (size_t)r0 * out->ld_s;
+        const void *xr = (const char *)x + (size_t)r0 * ldx * es;
+#define MX_Q(F, B)                                                                                                   \
+    IRIS_LAUNCH((mx_quantize_kernel<F, B>), grid, dim3(NT), 0, iris_stream(), q, s, out->ld_q, out->ld_s, xr, ldx,   \
+                cols, cpr, n, vec)
+        if (out->fmt == IRIS_MX_FP8) {
+            if (is_bf16) MX_Q(IRIS_MX_FP8, true);
+            else MX_Q(IRIS_MX_FP8, false);
+        } else {
+            if (is_bf16) MX_Q(IRIS_MX_FP4, true);
+            else MX_Q(IRIS_MX_FP4, false);
+        }
+#undef MX_Q
+        if (iris_launch_check("mx_quantize_kernel")) return -1;
+    }
+    return 0;
+}
+
+int iris_hip_mx_dequantize(void *y, int is_bf16, int ldy, const iris_mx_t *a, int rows, int cols) {
+    if (rows <= 0 || cols <= 0) return 0;
+    if (!a || !y) return iris_set_error("mx_dequantize: null argument");
+    if (check_mx("mx_dequantize", *a, cols)) return -1;
+    if (ldy < cols) return iris_set_error("mx_dequantize: row stride %d of %d columns", ldy, cols);
+    if (!iris_hip_available()) return -1;
+    const int es = is_bf16 ? 2 : 4;
+    const uint32_t cpr = (uint32_t)(cols + 7) / 8;
+    const bool vec = rows16(y, ldy, es);
+    for (int r0 = 0, nr; r0 < rows; r0 += nr) {
+        nr = rows - r0 < rows_per_launch(cpr) ? rows - r0 : rows_per_launch(cpr);
+        const uint32_t n = (uint32_t)nr * cpr;
+        const dim3 grid((n + NT - 1) / NT);
+        const uint8_t *q = a->q + (size_t)r0 * a->ld_q, *s = a->s + (size_t)r0 * a->ld_s;
+        void *yr = (char *)y + (size_t)r0 * ldy * es;
+#define MX_D(F, B)                                                                                                   \
+    IRIS_LAUNCH((mx_dequantize_kernel<F, B>), grid, dim3(NT), 0, iris_stream(), yr, ldy, q, s, a->ld_q, a->ld_s,     \
+                cols, cpr, n, vec)
+        if (a->fmt == IRIS_MX_FP8) {
+            if (is_bf16) MX_D(IRIS_MX_FP8, true);
+            else MX_D(IRIS_MX_FP8, false);
+        } else {
+            if (is_bf16) MX_D(IRIS_MX_FP4, true);
+            else MX_D(IRIS_MX_FP4, false);
+        }
+#undef MX_D
+        if (iris_launch_check("mx_dequantize_kernel")) return -1;
+    }
+    return 0;
+}
+
+}  /* extern "C" */
+
+namespace {
+template <int FMT, int DT> void launch_norm(const NormParams &P, int rows) {
+    const int r = (P.cols_pad / 8 + NT - 1) / NT;
+#define MX_N(R) IRIS_LAUNCH((mx_rmsnorm_kernel<FMT, DT, R>), dim3(rows), dim3(NT), 0, iris_stream(), P)
+    if (r == 1) MX_N(1);
+    else if (r == 2) MX_N(2);
+    else if (r <= 4) MX_N(4);
+    else MX_N(0);
+#undef MX_N
+}
+}  // namespace
+
+extern "C" int iris_hip_mx_rmsnorm(const iris_mx_norm_t *a) {
+    if (!a) return iris_set_error("mx_rmsnorm: null argument");
+    if (a->rows <= 0 || a->cols <= 0) return 0;
+    if (!a->x || !a->w || (a->d && !a->x_out) || (a->gate && !a->d)) return iris_set_error("mx_rmsnorm: null argument");
+    if (check_mx("mx_rmsnorm", a->out, a->cols)) return -1;
+    if (a->d && a->x_out == a->x && a->ldxo != a->ldx)
+        return iris_set_error("mx_rmsnorm: in place with row strides %d and %d", a->ldx, a->ldxo);
+    if (a->ldx < a->cols || (a->d && (a->ldd < a->cols || a->ldxo < a->cols)))
+        return iris_set_error("mx_rmsnorm: row strides %d, %d, %d of %d columns", a->ldx, a->ldd, a->ldxo, a->cols);
+    if (!iris_hip_available()) return -1;
+    NormParams P;
+    P.x = a->x; P.gate = a->gate; P.w = a->w; P.scale = a->scale; P.d = a->d; P.x_out = a->x_out;
+    P.q = a->out.q; P.s = a->out.s; P.ld_q = a->out.ld_q; P.ld_s = a->out.ld_s;
+    P.ldx = a->ldx; P.ldd = a->ldd; P.ldxo = a->ldxo;
+    P.cols = a->cols; P.cols_pad = pad_to(a->cols, 128); P.eps = a->eps;
+    P.vx = rows16(a->x, a->ldx, 4);
+    P.vd = rows16(a->d, a->ldd, a->d_bf16 ? 2 : 4);
+    P.vo = rows16(a->x_out, a->ldxo, 4);
+    const int dt = !a->d ? 0 : a->d_bf16 ? 2 : 1;
+    if (a->out.fmt == IRIS_MX_FP8) {
+        if (dt == 0) launch_norm<IRIS_MX_FP8, 0>(P, a->rows);
+        else if (dt == 1) launch_norm<IRIS_MX_FP8, 1>(P, a->rows);
+        else launch_norm<IRIS_MX_FP8, 2>(P, a->rows);
+    } else {
+        if (dt == 0) launch_norm<IRIS_MX_FP4, 0>(P, a->rows);
+        else if (dt == 1) launch_norm<IRIS_MX_FP4, 1>(P, a->rows);
+        else launch_norm<IRIS_MX_FP4, 2>(P, a->rows);
+    }
+    return iris_launch_check("mx_rmsnorm_kernel");
+}
+
+extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_bytes) {
+    if (!p) return iris_set_error("mx_gemm: null problem");
+    if (p->M <= 0 || p->N <= 0) return 0;
+    if (p->K <= 0) return iris_set_error("mx_gemm: K %d", p->K);
+    if (check_mx("mx_gemm A", p->A, p->K) || check_mx("mx_gemm W", p->W, p->K)) return -1;
+    if (p->W.fmt != IRIS_MX_FP4) return iris_set_error("mx_gemm: weights of format %d, not IRIS_MX_FP4", p->W.fmt);
+    const bool swiglu = p->epi == IRIS_EPI_SWIGLU, mx = swiglu && p->mx_out.q;
+    if (!swiglu && p->epi != IRIS_EPI_F32 && p->epi != IRIS_EPI_BF16 && p->epi != IRIS_EPI_GATED_ADD &&
+        p->epi != IRIS_EPI_ADD)
+        return iris_set_error("mx_gemm: epilogue %d", p->epi);
+    if (swiglu && (p->N % 64 || p->vec)) return iris_set_error("mx_gemm: SWIGLU needs N %% 64 == 0 (%d) and no vec", p->N);
+    if (!swiglu && p->mx_out.q) return iris_set_error("mx_gemm: mx_out is for SWIGLU");
+    const int nout = swiglu ? p->N / 2 : p->N;
+    if (mx ? check_mx("mx_gemm output", p->mx_out, nout) : !p->out ? iris_set_error("mx_gemm: null output") : 0) return -1;
+    if (!mx && p->ldo < nout) return iris_set_error("mx_gemm: output row stride %d of %d columns", p->ldo, nout);
+    if (!iris_hip_available()) return -1;
+    (void)ws;
+    (void)ws_bytes;
+    MxGemm P;
+    P.aq = p->A.q; P.as = p->A.s; P.lda = p->A.ld_q; P.ldas = p->A.ld_s;
+    P.wq = p->W.q; P.ws = p->W.s; P.ldw = p->W.ld_q; P.ldws = p->W.ld_s;
+    P.out = p->out; P.vec = p->vec; P.M = p->M; P.N = p->N; P.ldo = p->ldo; P.epi = p->epi;
+    P.steps = pad_to(p->K, 128) / 128;
+    P.oq = mx ? p->mx_out.q : nullptr; P.os = p->mx_out.s;
+    P.ldoq = p->mx_out.ld_q; P.ldos = p->mx_out.ld_s; P.ofmt = p->mx_out.fmt;
+    constexpr int FM = 4, FN = 4;
+    const long long tiles = (long long)((p->M + 16 * FM - 1) / (16 * FM)) * ((p->N + 16 * FN - 1) / (16 * FN));
+    if (tiles > 0x7fffffffLL) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
+    if (p->A.fmt == IRIS_MX_FP8)
+        IRIS_LAUNCH((mx_gemm_direct_kernel<IRIS_MX_FP8, FM, FN>), dim3((unsigned)tiles), dim3(512), 0, iris_stream(), P);
+    else
+        IRIS_LAUNCH((mx_gemm_direct_kernel<IRIS_MX_FP4, FM, FN>), dim3((unsigned)tiles), dim3(512), 0, iris_stream(), P);
+    return iris_launch_check("mx_gemm_direct_kernel");
+}
