@@ -484,6 +484,318 @@ template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm
     }
 }
 
+/* ---- product on LDS tiles ----
+ * 8 waves, 4 along M x 2 along N, block tile BM x BN, two LDS stages of one K
+ * step each: 128 columns with e4m3 A (rows of 128 and 64 bytes), 256 with
+ * e2m1 A (128 and 128 bytes). 16-byte chunks of a row are stored XORed with
+ * its row number, so that the loads, which place 64 lanes' 16 bytes one after
+ * the other, give fragment reads without bank conflicts. Waves w and w + 4
+ * share a SIMD: group 0 (waves 0..3) and group 1 take turns, one reading a K
+ * step's fragments while the other runs its matrix instructions (phases as
+ * described at the loop).
+ * Scales: 16 bytes of a row are 512 columns. They are loaded into LDS as they
+ * are (A's by group 0, W's by group 1), then a lane transposes the 4 x 4 bytes
+ * of a row so that the bytes of lane group g (block g of each 128 columns)
+ * make one word; a fragment's lane reads its word once per 512 columns and the
+ * instruction picks the byte. */
+constexpr int waitcnt_imm(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
+typedef __attribute__((address_space(3))) void lds_void;
+constexpr int GROUP_M = 8;
+
+struct MxTiles {
+    int tiles_m, tiles_n, per_xcd;
+};
+
+template <int OP, int AF>
+__device__ __forceinline__ f32x4 mx_mfma_op(const u32x4 &w, const i32x8 &a, const f32x4 &c, int sw, int sa) {
+    const i32x8 w8 = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, a, c, 4, AF == IRIS_MX_FP8 ? 0 : 4, OP, sw, OP, sa);
+}
+
+/* byte j of word i to byte i of word j */
+__device__ __forceinline__ u32x4 bytes4x4(const u32x4 &x) {
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400), b = __builtin_amdgcn_perm(x[1], x[0], 0x07030602);
+    const uint32_t c = __builtin_amdgcn_perm(x[3], x[2], 0x05010400), d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602);
+    return (u32x4){__builtin_amdgcn_perm(c, a, 0x05040100), __builtin_amdgcn_perm(c, a, 0x07060302),
+                   __builtin_amdgcn_perm(d, b, 0x05040100), __builtin_amdgcn_perm(d, b, 0x07060302)};
+}
+
+template <int V> struct Const {
+    static constexpr int value = V;
+};
+
+template <int AF, bool SPLIT, int BM, int BN>
+__global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const MxTiles T) {
+    constexpr bool F8 = AF == IRIS_MX_FP8;
+    constexpr int WROW = F8 ? 64 : 128, KS = F8 ? 1 : 2, PER = 4 / KS;   /* K steps per 512 columns */
+    constexpr int TWM = BM / 4, TWN = BN / 2, FM = TWM / 16, FN = TWN / 16;
+    constexpr int A_BYTES = BM * 128, STAGE = A_BYTES + BN * WROW;
+    constexpr int A_DMA = BM / 32, W_ROWS = 1024 / WROW, W_DMA = BN / W_ROWS / 4;   /* loads per wave of a group */
+    __shared__ __attribute__((aligned(16))) uint8_t lds0[STAGE];
+    __shared__ __attribute__((aligned(16))) uint8_t lds1[STAGE];
+    __shared__ u32x4 raw[BM + BN];
+    __shared__ u32x4 scl[BM + BN];
+    const int L = (int)(blockIdx.x & 7) * T.per_xcd + (int)(blockIdx.x >> 3);
+    if (L >= T.tiles_m * T.tiles_n) return;
+    const int first_m = L / (GROUP_M * T.tiles_n) * GROUP_M, gsz = min(T.tiles_m - first_m, GROUP_M);
+    const int tg = L - first_m * T.tiles_n, tn = tg / gsz;
+    const int m0 = (first_m + tg - tn * gsz) * BM, n0 = tn * BN;
+
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = wave >> 2, gw = wave & 3;
+    const int wm = wave >> 1, wn = wave & 1;
+
+    /* rows past the end read as zeros */
+    const __amdgpu_buffer_rsrc_t a_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(P.aq + (size_t)m0 * P.lda), (short)0, min(BM, P.M - m0) * P.lda, 0x00020000);
+    const __amdgpu_buffer_rsrc_t w_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(P.wq + (size_t)n0 * P.ldw), (short)0, min(BN, P.N - n0) * P.ldw, 0x00020000);
+    /* load j of rows of 128 bytes covers rows 8 j .., lane l row 8 j + l / 8,
+     * place l % 8, chunk place ^ (row / 2 % 8): by the parity of j. Rows of 64
+     * bytes: rows 16 j .., row l / 4, chunk place ^ (row / 2 % 4). */
+    auto hidden_lane = [&]() {   /* places are computed anew in each step: registers are short */
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        return l;
+    };
+    /* row row0 + l / 8 of load j. A step of 256 columns of which the row has
+     * only 128 reads those twice, not what lies behind the row. */
+    const int nk = (P.steps + KS - 1) / KS, ng = (P.steps + 3) / 4;
+    auto voff128 = [](int l, int row0, int ld, int j, int chunks) {
+        return (row0 + (l >> 3)) * ld + ((((l & 7) ^ ((4 * (j & 1) + (l >> 4)) & 7)) & chunks) << 4);
+    };
+    auto chunks_of = [&](int kt) { return !F8 && 2 * kt + 1 >= P.steps ? 3 : 7; };
+    auto dma_a = [&](uint8_t *stage, int kt) {
+        const int l = hidden_lane(), j0 = gw * A_DMA, ch = chunks_of(kt);
+        const int v[2] = {voff128(l, j0 * 8, P.lda, j0, ch), voff128(l, j0 * 8, P.lda, j0 + 1, ch)};
+#pragma unroll
+        for (int i = 0; i < A_DMA; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, (lds_void *)(stage + (j0 + i) * 1024), 16,
+                                                     v[i & 1] + i * 8 * P.lda, kt * 128, 0, 0);
+    };
+    auto dma_w = [&](uint8_t *stage, int kt) {
+        const int l = hidden_lane(), j0 = gw * W_DMA;
+        int v[2];
+        if constexpr (F8) v[0] = v[1] = (j0 * 16 + (l >> 2)) * P.ldw + (((l & 3) ^ ((l >> 3) & 3)) << 4);
+        else v[0] = voff128(l, j0 * 8, P.ldw, j0, chunks_of(kt)), v[1] = voff128(l, j0 * 8, P.ldw, j0 + 1, chunks_of(kt));
+#pragma unroll
+        for (int i = 0; i < W_DMA; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(w_rsrc, (lds_void *)(stage + A_BYTES + (j0 + i) * 1024), 16,
+                                                     v[i & 1] + i * W_ROWS * P.ldw, kt * WROW, 0, 0);
+    };
+    /* scales of 512 columns: lane l of wave gw row 64 gw + l of its group's operand */
+    const int srow = gw * 64;
+    const bool has_rows = srow < (grp ? BN : BM);
+    const __amdgpu_buffer_rsrc_t s_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(grp ? P.ws + (size_t)n0 * P.ldws : P.as + (size_t)m0 * P.ldas), (short)0,
+        grp ? min(BN, P.N - n0) * P.ldws : min(BM, P.M - m0) * P.ldas, 0x00020000);
+    const int s_at = (grp ? BM : 0) + srow;
+    auto scl_load = [&](int g) {
+        const int l = hidden_lane();
+        if (has_rows)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(s_rsrc, (lds_void *)(raw + s_at), 16,
+                                                     (srow + l) * (grp ? P.ldws : P.ldas), g * 16, 0, 0);
+    };
+    auto scl_put = [&]() {
+        const int l = hidden_lane();
+        if (has_rows) scl[s_at + l] = bytes4x4(raw[s_at + l]);
+    };
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    i32x8 a8[FM];                /* e4m3: 128 columns */
+    u32x4 a[2][FM], w[KS][FN];   /* e2m1: two times 128 */
+    int sa[FM], sw[FN];
+    /* rows 16 apart are stored alike, chunk 4 + lg is chunk lg XOR 4 */
+    auto frags = [&](const uint8_t *stage) {
+        const int l = hidden_lane(), r = l & 15, c = l >> 4;
+        const int pa = wm * TWM * 128 + r * 128 + ((c ^ (r >> 1)) << 4);
+        const int pw = A_BYTES + wn * TWN * WROW + r * WROW + ((c ^ (F8 ? (r >> 1) & 3 : r >> 1)) << 4);
+#pragma unroll
+        for (int i = 0; i < FM; i++) {
+            const u32x4 x = *(const u32x4 *)(stage + pa + i * 2048), y = *(const u32x4 *)(stage + (pa ^ 64) + i * 2048);
+            if constexpr (F8) {
+                a8[i] = (i32x8){(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+            } else {
+                a[0][i] = x;
+                a[1][i] = y;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < KS; h++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) w[h][j] = *(const u32x4 *)(stage + (h ? pw ^ 64 : pw) + j * 16 * WROW);
+    };
+    auto scales = [&]() {
+        const int l = hidden_lane(), at = (l & 15) * 16 + (l >> 4) * 4, pa = wm * TWM * 16 + at, pw = (BM + wn * TWN) * 16 + at;
+#pragma unroll
+        for (int i = 0; i < FM; i++) sa[i] = *(const int *)((const uint8_t *)scl + pa + i * 256);
+#pragma unroll
+        for (int j = 0; j < FN; j++) sw[j] = *(const int *)((const uint8_t *)scl + pw + j * 256);
+    };
+    /* half h of a K step: e2m1, its 128 columns; e4m3, half of the rows' tiles */
+    auto mfmas = [&](auto s_, auto h_, bool there) {
+        constexpr int S = decltype(s_)::value, H = decltype(h_)::value;
+        if constexpr (F8) {
+#pragma unroll
+            for (int i = H * FM / 2; i < (H + 1) * FM / 2; i++) {
+                i32x8 hi = a8[i], lo = a8[i];
+                if constexpr (SPLIT) mx_split(a8[i], hi, lo);
+#pragma unroll
+                for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma_op<S, AF>(w[0][j], hi, acc[i][j], sw[j], sa[i]);
+                if constexpr (SPLIT)
+#pragma unroll
+                    for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma_op<S, AF>(w[0][j], lo, acc[i][j], sw[j], sa[i]);
+            }
+        } else if (H == 0 || there) {
+#pragma unroll
+            for (int i = 0; i < FM; i++) {
+                const i32x8 x = {(int)a[H][i][0], (int)a[H][i][1], (int)a[H][i][2], (int)a[H][i][3], 0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma_op<2 * S + H, AF>(w[H < KS ? H : 0][j], x, acc[i][j], sw[j], sa[i]);
+            }
+        }
+    };
+    /* the compiler takes the scaled instruction for one that it may move past
+     * barriers and into branches, and then keeps a K step's operands for it */
+    auto pin = [&]() {
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) asm volatile("" ::"v"(acc[i][j]));
+    };
+#define WAIT(vm, lgkm)                                              \
+    do {                                                            \
+        __builtin_amdgcn_sched_barrier(0);                          \
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(vm, lgkm));          \
+        __builtin_amdgcn_sched_barrier(0);                          \
+    } while (0)
+    auto barrier = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    /* Phases between barriers: group 0 runs L(t), C(t) in phases 2t, 2t + 1,
+     * group 1 in phases 2t + 1, 2t + 2; L reads step t's fragments (stage t %
+     * 2), C runs its matrix instructions. Each group loads one operand:
+     *  - group 0 issues A of step t + 1 in L(t) into the other stage, which
+     *    both groups read before phase 2t, and waits for it at the end of C(t);
+     *  - group 1 issues W of step t + 2 in L(t) into the stage that it has
+     *    just read, behind a barrier in the middle of phase 2t + 1 (group 0,
+     *    which read step t in phase 2t, meets it inside C(t)), and waits for
+     *    it in L(t + 1).
+     * Scales of 512 columns are read in L of the first step of them, and
+     * those of the next 512 written in L of their last step. Past the last
+     * step the loads repeat it into a stage nothing reads again. */
+    auto step0 = [&](auto s_, auto last_, uint8_t *cur, uint8_t *nxt, int kt, int g) {
+        constexpr int S = decltype(s_)::value, LAST = decltype(last_)::value;
+        const bool there = F8 || !LAST || kt * 2 + 1 < P.steps;
+        if constexpr (S == PER - 1) {
+            if (g + 1 < ng) scl_put();
+        }
+        if constexpr (S == 0) scales();
+        frags(cur);
+        dma_a(nxt, min(kt + 1, nk - 1));
+        if constexpr (S == 0) {
+            if (g + 1 < ng) scl_load(g + 1);
+        }
+        WAIT(63, 0);
+        barrier();
+        mfmas(s_, Const<0>{}, there);
+        pin();
+        barrier();   /* group 1's reads of step kt are done */
+        mfmas(s_, Const<1>{}, there);
+        pin();
+        WAIT(0, 0);
+        barrier();
+    };
+    auto step1 = [&](auto s_, auto last_, uint8_t *cur, int kt, int g) {
+        constexpr int S = decltype(s_)::value, LAST = decltype(last_)::value;
+        const bool there = F8 || !LAST || kt * 2 + 1 < P.steps;
+        if constexpr (S == 0) scales();
+        frags(cur);
+        WAIT(0, 0);
+        barrier();   /* every wave of the group has read step kt */
+        dma_w(cur, min(kt + 2, nk - 1));
+        if constexpr (S == 0) {
+            if (g + 1 < ng) scl_load(g + 1);
+        }
+        if constexpr (S == PER - 1) {
+            if (g + 1 < ng) scl_put();
+            WAIT(63, 0);
+        }
+        barrier();
+        mfmas(s_, Const<0>{}, there);
+        mfmas(s_, Const<1>{}, there);
+        pin();
+        if (kt + 1 < nk) barrier();
+    };
+    scl_load(0);
+    if (grp) {
+        dma_w(lds0, 0);
+        WAIT(0, 0);
+        scl_put();
+        WAIT(0, 0);
+        barrier();
+        dma_w(lds1, min(1, nk - 1));
+        barrier();
+        const int whole = P.steps / 4;
+        for (int g = 0; g < whole; g++) {
+            step1(Const<0>{}, Const<0>{}, lds0, g * PER, g);
+            step1(Const<1>{}, Const<0>{}, lds1, g * PER + 1, g);
+            if constexpr (PER == 4) {
+                step1(Const<2>{}, Const<0>{}, lds0, g * PER + 2, g);
+                step1(Const<3>{}, Const<0>{}, lds1, g * PER + 3, g);
+            }
+        }
+        const int kt = whole * PER;
+        if (kt < nk) step1(Const<0>{}, Const<1>{}, lds0, kt, whole);
+        if (kt + 1 < nk) step1(Const<1>{}, Const<1>{}, lds1, kt + 1, whole);
+        if constexpr (PER == 4) {
+            if (kt + 2 < nk) step1(Const<2>{}, Const<1>{}, lds0, kt + 2, whole);
+        }
+    } else {
+        dma_a(lds0, 0);
+        WAIT(0, 0);
+        scl_put();
+        WAIT(0, 0);
+        barrier();
+        const int whole = P.steps / 4;
+        for (int g = 0; g < whole; g++) {
+            step0(Const<0>{}, Const<0>{}, lds0, lds1, g * PER, g);
+            step0(Const<1>{}, Const<0>{}, lds1, lds0, g * PER + 1, g);
+            if constexpr (PER == 4) {
+                step0(Const<2>{}, Const<0>{}, lds0, lds1, g * PER + 2, g);
+                step0(Const<3>{}, Const<0>{}, lds1, lds0, g * PER + 3, g);
+            }
+        }
+        const int kt = whole * PER;
+        if (kt < nk) step0(Const<0>{}, Const<1>{}, lds0, lds1, kt, whole);
+        if (kt + 1 < nk) step0(Const<1>{}, Const<1>{}, lds1, lds0, kt + 1, whole);
+        if constexpr (PER == 4) {
+            if (kt + 2 < nk) step0(Const<2>{}, Const<1>{}, lds0, lds1, kt + 2, whole);
+        }
+    }
+    WAIT(0, 0);   /* no load outstanding at exit */
+#undef WAIT
+    const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+        const int m = m0 + wm * TWM + i * 16 + lr;
+        if (P.epi == IRIS_EPI_SWIGLU) {
+#pragma unroll
+            for (int j = 0; j < FN; j += 4)
+                mx_store_swiglu(P, m, n0 + wn * TWN + j * 16, acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], aligned);
+        } else if (m < P.M) {
+#pragma unroll
+            for (int j = 0; j < FN; j++) mx_store4(P, m, n0 + wn * TWN + j * 16 + 4 * lg, acc[i][j], aligned);
+        }
+    }
+}
+
 /* ---- argument checks ---- */
 int pad_to(long long v, int to) { return (int)((v + to - 1) / to * to); }
 
@@ -644,6 +956,24 @@ extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_by
     P.steps = pad_to(p->K, 128) / 128;
     P.oq = mx ? p->mx_out.q : nullptr; P.os = p->mx_out.s;
     P.ldoq = p->mx_out.ld_q; P.ldos = p->mx_out.ld_s; P.ofmt = p->mx_out.fmt;
+    const bool far = (long long)(p->A.ld_q > p->W.ld_q ? p->A.ld_q : p->W.ld_q) * 256 > 0x7fffffffLL;
+    if (p->M > 128 && !far) {
+        MxTiles T;
+        T.tiles_m = (p->M + 255) / 256;
+        T.tiles_n = (p->N + 255) / 256;
+        const long long total = (long long)T.tiles_m * T.tiles_n;
+        if (total > 0x7fffffff / 2) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
+        T.per_xcd = (int)((total + 7) / 8);
+        const bool exact = p->epi != IRIS_EPI_BF16 && !swiglu;
+        const dim3 grid(8 * T.per_xcd);
+        if (p->A.fmt == IRIS_MX_FP4)
+            IRIS_LAUNCH((mx_gemm_tile_kernel<IRIS_MX_FP4, false, 256, 256>), grid, dim3(512), 0, iris_stream(), P, T);
+        else if (exact)
+            IRIS_LAUNCH((mx_gemm_tile_kernel<IRIS_MX_FP8, true, 256, 256>), grid, dim3(512), 0, iris_stream(), P, T);
+        else
+            IRIS_LAUNCH((mx_gemm_tile_kernel<IRIS_MX_FP8, false, 256, 256>), grid, dim3(512), 0, iris_stream(), P, T);
+        return iris_launch_check("mx_gemm_tile_kernel");
+    }
     constexpr int FM = 4, FN = 4;
     const long long tiles = (long long)((p->M + 16 * FM - 1) / (16 * FM)) * ((p->N + 16 * FN - 1) / (16 * FN));
     if (tiles > 0x7fffffffLL) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
