@@ -520,6 +520,8 @@ __device__ __forceinline__ u32x4 bytes4x4(const u32x4 &x) {
                    __builtin_amdgcn_perm(d, b, 0x05040100), __builtin_amdgcn_perm(d, b, 0x07060302)};
 }
 
+__device__ __forceinline__ bool rows16_ok(const void *p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0; }
+
 template <int V> struct Const {
     static constexpr int value = V;
 };
@@ -781,18 +783,86 @@ __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const
     }
     WAIT(0, 0);   /* no load outstanding at exit */
 #undef WAIT
+    /* Whole tiles of 16-bit or microscaled output leave through LDS, two of a
+     * wave's 16-row tiles at a time, so that a row's part of a wave (256, 128
+     * or 64 bytes) is written by neighbouring lanes: 8-byte stores of 16 rows
+     * each took 10 us more of 4096 x 4096 x 2560. */
+    const bool full = m0 + BM <= P.M && n0 + BN <= P.N;
+    uint8_t *const st = (grp ? lds1 : lds0) + gw * 8192;
+    static_assert(STAGE >= 4 * 8192, "a wave's part of a stage");
+    if (full && P.epi == IRIS_EPI_BF16 && rows16_ok(P.out, P.ldo)) {
+        __syncthreads();   /* every wave is done with the stages */
+#pragma unroll
+        for (int ip = 0; ip < FM; ip += 2) {
+#pragma unroll
+            for (int j = 0; j < FN; j++) {
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (P.vec)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) v[r] = P.vec[n0 + wn * TWN + j * 16 + 4 * lg + r];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const f32x4 x = acc[ip + i][j];
+                    const int row = i * 16 + lr;
+                    *(uint2 *)(st + row * (TWN * 2) + (((2 * j + (lg >> 1)) ^ (row & (FN * 2 - 1))) << 4) + (lg & 1) * 8) =
+                        make_uint2((uint32_t)f2bf_hw(x[0] + v[0]) | (uint32_t)f2bf_hw(x[1] + v[1]) << 16,
+                                   (uint32_t)f2bf_hw(x[2] + v[2]) | (uint32_t)f2bf_hw(x[3] + v[3]) << 16);
+                }
+            }
+            uint16_t *const out = (uint16_t *)P.out + (size_t)(m0 + wm * TWM + ip * 16) * P.ldo + n0 + wn * TWN;
+            constexpr int CPR = FN * 2;
+#pragma unroll
+            for (int c = lane; c < 32 * CPR; c += 64) {
+                const int row = c / CPR, ch = c % CPR;
+                *(u32x4 *)(out + (size_t)row * P.ldo + ch * 8) = *(const u32x4 *)(st + row * (TWN * 2) + ((ch ^ (row & (CPR - 1))) << 4));
+            }
+        }
+        return;
+    }
+    if (full && P.epi == IRIS_EPI_SWIGLU && !P.oq && rows16_ok(P.out, P.ldo)) {
+        __syncthreads();
+#pragma unroll
+        for (int ip = 0; ip < FM; ip += 2) {
+#pragma unroll
+            for (int j = 0; j < FN / 4; j++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const f32x4 g = acc[ip + i][4 * j + h], u = acc[ip + i][4 * j + 2 + h];
+                        uint16_t y[4];
+#pragma unroll
+                        for (int r = 0; r < 4; r++) y[r] = f2bf_hw(silu_fast(g[r]) * u[r]);
+                        const int row = i * 16 + lr;
+                        *(uint2 *)(st + row * TWN + (((4 * j + 2 * h + (lg >> 1)) ^ (row & (FN - 1))) << 4) + (lg & 1) * 8) =
+                            make_uint2((uint32_t)y[0] | (uint32_t)y[1] << 16, (uint32_t)y[2] | (uint32_t)y[3] << 16);
+                    }
+            uint16_t *const out = (uint16_t *)P.out + (size_t)(m0 + wm * TWM + ip * 16) * P.ldo + (n0 + wn * TWN) / 2;
+            constexpr int CPR = FN;
+#pragma unroll
+            for (int c = lane; c < 32 * CPR; c += 64) {
+                const int row = c / CPR, ch = c % CPR;
+                *(u32x4 *)(out + (size_t)row * P.ldo + ch * 8) = *(const u32x4 *)(st + row * TWN + ((ch ^ (row & (CPR - 1))) << 4));
+            }
+        }
+        return;
+    }
     const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
+    if (P.epi == IRIS_EPI_SWIGLU) {
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j += 4)
+                mx_store_swiglu(P, m0 + wm * TWM + i * 16 + lr, n0 + wn * TWN + j * 16, acc[i][j], acc[i][j + 1],
+                                acc[i][j + 2], acc[i][j + 3], aligned);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < FM; i++) {
         const int m = m0 + wm * TWM + i * 16 + lr;
-        if (P.epi == IRIS_EPI_SWIGLU) {
-#pragma unroll
-            for (int j = 0; j < FN; j += 4)
-                mx_store_swiglu(P, m, n0 + wn * TWN + j * 16, acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], aligned);
-        } else if (m < P.M) {
+        if (m < P.M)
 #pragma unroll
             for (int j = 0; j < FN; j++) mx_store4(P, m, n0 + wn * TWN + j * 16 + 4 * lg, acc[i][j], aligned);
-        }
     }
 }
 
