@@ -294,13 +294,20 @@ __device__ __forceinline__ f32x4 mx_mfma(const u32x4 &w, const i32x8 &a, const f
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, a, c, 4, AF == IRIS_MX_FP8 ? 0 : 4, 0, sw, 0, sa);
 }
 
+/* of e2m1 codes, scales in byte OP */
+template <int OP>
+__device__ __forceinline__ f32x4 mx_mfma4(const u32x4 &w, const i32x8 &a, const f32x4 &c, int sw, int sa) {
+    const i32x8 w8 = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, a, c, 4, 4, OP, sw, OP, sa);
+}
+
 /* e4m3 codes of magnitude 2 and more (bit 6 set), and the others */
 __device__ __forceinline__ void mx_split(const i32x8 &a, i32x8 &hi, i32x8 &lo) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const uint32_t big = (((uint32_t)a[i] >> 6) & 0x01010101u) * 255u;
-        hi[i] = (int)((uint32_t)a[i] & big);
-        lo[i] = (int)((uint32_t)a[i] & ~big);
+        const uint32_t x = (uint32_t)a[i], big = ((x >> 6) & 0x01010101u) * 255u;
+        hi[i] = (int)(x & big);
+        lo[i] = (int)(x & ~big);
     }
 }
 
@@ -485,19 +492,20 @@ template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm
 }
 
 /* ---- product on LDS tiles ----
- * 8 waves, 4 along M x 2 along N, block tile BM x BN, two LDS stages of one K
- * step each: 128 columns with e4m3 A (rows of 128 and 64 bytes), 256 with
- * e2m1 A (128 and 128 bytes). 16-byte chunks of a row are stored XORed with
+ * 8 waves, 4 along M x 2 along N, block tile BM x BN. LDS holds two stages of
+ * A and two of W, rows of 128 bytes (e4m3: 128 columns, one K step; e2m1: 256):
+ * a load costs the CU's address and cache path 1.5 ns per row it touches, 128
+ * bytes or less, and with rows of 64 bytes that path, not the matrix
+ * instructions, took the time. 16-byte chunks of a row are stored XORed with
  * its row number, so that the loads, which place 64 lanes' 16 bytes one after
  * the other, give fragment reads without bank conflicts. Waves w and w + 4
- * share a SIMD: group 0 (waves 0..3) and group 1 take turns, one reading a K
- * step's fragments while the other runs its matrix instructions (phases as
- * described at the loop).
+ * share a SIMD: group 0 (waves 0..3, the tile's upper half) and group 1 take
+ * turns, one reading a K step's fragments while the other runs its matrix
+ * instructions (phases as described at the loop).
  * Scales: 16 bytes of a row are 512 columns. They are loaded into LDS as they
- * are (A's by group 0, W's by group 1), then a lane transposes the 4 x 4 bytes
- * of a row so that the bytes of lane group g (block g of each 128 columns)
- * make one word; a fragment's lane reads its word once per 512 columns and the
- * instruction picks the byte. */
+ * are, then a lane transposes the 4 x 4 bytes of a row so that the bytes of
+ * lane group g (block g of each 128 columns) make one word; a fragment's lane
+ * reads its word once per 512 columns and shifts it by a byte per 128. */
 constexpr int waitcnt_imm(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
 typedef __attribute__((address_space(3))) void lds_void;
 constexpr int GROUP_M = 8;
@@ -506,10 +514,20 @@ struct MxTiles {
     int tiles_m, tiles_n, per_xcd;
 };
 
-template <int OP, int AF>
-__device__ __forceinline__ f32x4 mx_mfma_op(const u32x4 &w, const i32x8 &a, const f32x4 &c, int sw, int sa) {
-    const i32x8 w8 = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, a, c, 4, AF == IRIS_MX_FP8 ? 0 : 4, OP, sw, OP, sa);
+/* 64 lanes' 16 bytes from a buffer to LDS, one after the other from place at on
+ * (rows past the buffer's end: zeros). Not the builtin: before reads of one
+ * stage the compiler waits for the builtin's loads into the others too, which
+ * takes the ring's depth away. The caller waits (vmcnt) before a barrier. */
+__device__ __forceinline__ uint32_t lds_at(const void *p) { return (uint32_t)(uintptr_t)(const lds_void *)p; }
+__device__ __forceinline__ void load_lds16(const u32x4 &rsrc, uint32_t at, int voff, int soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 ::"s"(at), "v"(voff), "s"(rsrc), "s"(soff)
+                 : "memory");
+}
+__device__ __forceinline__ u32x4 buffer_of(const void *p, int bytes) {
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    return (u32x4){(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)),
+                   (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
 }
 
 /* byte j of word i to byte i of word j */
@@ -529,12 +547,12 @@ template <int V> struct Const {
 template <int AF, bool SPLIT, int BM, int BN>
 __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const MxTiles T) {
     constexpr bool F8 = AF == IRIS_MX_FP8;
-    constexpr int WROW = F8 ? 64 : 128, KS = F8 ? 1 : 2, PER = 4 / KS;   /* K steps per 512 columns */
+    constexpr int KS = F8 ? 1 : 2, PER = 4 / KS;   /* 128 columns per step, steps per 512 columns */
     constexpr int TWM = BM / 4, TWN = BN / 2, FM = TWM / 16, FN = TWN / 16;
-    constexpr int A_BYTES = BM * 128, STAGE = A_BYTES + BN * WROW;
-    constexpr int A_DMA = BM / 32, W_ROWS = 1024 / WROW, W_DMA = BN / W_ROWS / 4;   /* loads per wave of a group */
-    __shared__ __attribute__((aligned(16))) uint8_t lds0[STAGE];
-    __shared__ __attribute__((aligned(16))) uint8_t lds1[STAGE];
+    constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128;
+    constexpr int A_LD = BM / 64, W_LD = BN / 32 / (F8 ? 2 : 1);   /* loads of a wave: half of A's rows; W's per step */
+    constexpr int SC_LD = (BM + BN + 255) / 256;                  /* and of scales */
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * (A_BYTES + W_BYTES)];
     __shared__ u32x4 raw[BM + BN];
     __shared__ u32x4 scl[BM + BN];
     const int L = (int)(blockIdx.x & 7) * T.per_xcd + (int)(blockIdx.x >> 3);
@@ -548,59 +566,54 @@ __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const
     const int wm = wave >> 1, wn = wave & 1;
 
     /* rows past the end read as zeros */
-    const __amdgpu_buffer_rsrc_t a_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)(P.aq + (size_t)m0 * P.lda), (short)0, min(BM, P.M - m0) * P.lda, 0x00020000);
-    const __amdgpu_buffer_rsrc_t w_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)(P.wq + (size_t)n0 * P.ldw), (short)0, min(BN, P.N - n0) * P.ldw, 0x00020000);
-    /* load j of rows of 128 bytes covers rows 8 j .., lane l row 8 j + l / 8,
-     * place l % 8, chunk place ^ (row / 2 % 8): by the parity of j. Rows of 64
-     * bytes: rows 16 j .., row l / 4, chunk place ^ (row / 2 % 4). */
+    const u32x4 a_rsrc = buffer_of(P.aq + (size_t)m0 * P.lda, min(BM, P.M - m0) * P.lda);
+    const u32x4 w_rsrc = buffer_of(P.wq + (size_t)n0 * P.ldw, min(BN, P.N - n0) * P.ldw);
+    const u32x4 as_rsrc = buffer_of(P.as + (size_t)m0 * P.ldas, min(BM, P.M - m0) * P.ldas);
+    const u32x4 ws_rsrc = buffer_of(P.ws + (size_t)n0 * P.ldws, min(BN, P.N - n0) * P.ldws);
+    const int nk = (P.steps + KS - 1) / KS, nw = (P.steps + 1) / 2, ng = (P.steps + 3) / 4;
+    const uint32_t at0 = lds_at(lds), raw0 = lds_at(raw);
     auto hidden_lane = [&]() {   /* places are computed anew in each step: registers are short */
         int l = lane;
         asm volatile("" : "+v"(l));
         return l;
     };
-    /* row row0 + l / 8 of load j. A step of 256 columns of which the row has
-     * only 128 reads those twice, not what lies behind the row. */
-    const int nk = (P.steps + KS - 1) / KS, ng = (P.steps + 3) / 4;
-    auto voff128 = [](int l, int row0, int ld, int j, int chunks) {
-        return (row0 + (l >> 3)) * ld + ((((l & 7) ^ ((4 * (j & 1) + (l >> 4)) & 7)) & chunks) << 4);
+    /* A load covers 8 rows: lane l row l / 8, place l % 8, chunk place ^ (row /
+     * 2 % 8), which depends on the load by its parity. Of 256 columns that the
+     * row has only half of, that half is read twice, not what lies behind. */
+    auto place = [](int l, int ld, int row0, int par, int chunks) {
+        return (row0 + (l >> 3)) * ld + ((((l & 7) ^ ((4 * par + (l >> 4)) & 7)) & chunks) << 4);
     };
-    auto chunks_of = [&](int kt) { return !F8 && 2 * kt + 1 >= P.steps ? 3 : 7; };
-    auto dma_a = [&](uint8_t *stage, int kt) {
-        const int l = hidden_lane(), j0 = gw * A_DMA, ch = chunks_of(kt);
-        const int v[2] = {voff128(l, j0 * 8, P.lda, j0, ch), voff128(l, j0 * 8, P.lda, j0 + 1, ch)};
-#pragma unroll
-        for (int i = 0; i < A_DMA; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, (lds_void *)(stage + (j0 + i) * 1024), 16,
-                                                     v[i & 1] + i * 8 * P.lda, kt * 128, 0, 0);
+    /* half h of A's rows, step kt, into stage dst % 2 */
+    auto load_a = [&](int h, int kt, int dst, int l, int i) {
+        const int j0 = h * (BM / 16) + gw * A_LD, par = i & 1;
+        const int ch = !F8 && 2 * kt + 1 >= P.steps ? 3 : 7;
+        load_lds16(a_rsrc, at0 + (dst & 1) * A_BYTES + (j0 + i) * 1024,
+                   place(l, P.lda, (j0 + par) * 8, par, ch) + (i - par) * 8 * P.lda, kt * 128);
     };
-    auto dma_w = [&](uint8_t *stage, int kt) {
-        const int l = hidden_lane(), j0 = gw * W_DMA;
-        int v[2];
-        if constexpr (F8) v[0] = v[1] = (j0 * 16 + (l >> 2)) * P.ldw + (((l & 3) ^ ((l >> 3) & 3)) << 4);
-        else v[0] = voff128(l, j0 * 8, P.ldw, j0, chunks_of(kt)), v[1] = voff128(l, j0 * 8, P.ldw, j0 + 1, chunks_of(kt));
-#pragma unroll
-        for (int i = 0; i < W_DMA; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(w_rsrc, (lds_void *)(stage + A_BYTES + (j0 + i) * 1024), 16,
-                                                     v[i & 1] + i * W_ROWS * P.ldw, kt * WROW, 0, 0);
+    /* W's rows, 256 columns kw, into stage dst % 2; e4m3: half s of the loads */
+    auto load_w = [&](int kw, int dst, int s, int l, int i) {
+        const int j0 = (s * 4 + gw) * W_LD, par = i & 1;
+        const int ch = 2 * kw + 1 >= P.steps ? 3 : 7;
+        load_lds16(w_rsrc, at0 + 2 * A_BYTES + (dst & 1) * W_BYTES + (j0 + i) * 1024,
+                   place(l, P.ldw, (j0 + par) * 8, par, ch) + (i - par) * 8 * P.ldw, kw * 128);
     };
-    /* scales of 512 columns: lane l of wave gw row 64 gw + l of its group's operand */
-    const int srow = gw * 64;
-    const bool has_rows = srow < (grp ? BN : BM);
-    const __amdgpu_buffer_rsrc_t s_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)(grp ? P.ws + (size_t)n0 * P.ldws : P.as + (size_t)m0 * P.ldas), (short)0,
-        grp ? min(BN, P.N - n0) * P.ldws : min(BM, P.M - m0) * P.ldas, 0x00020000);
-    const int s_at = (grp ? BM : 0) + srow;
-    auto scl_load = [&](int g) {
+    /* scales of 512 columns g: wave w of group 1 rows 64 (w + 4 i) .. of A's and then W's */
+    auto load_scales = [&](int g) {
         const int l = hidden_lane();
-        if (has_rows)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(s_rsrc, (lds_void *)(raw + s_at), 16,
-                                                     (srow + l) * (grp ? P.ldws : P.ldas), g * 16, 0, 0);
+#pragma unroll
+        for (int i = 0; i < SC_LD; i++) {
+            const int r = (gw + 4 * i) * 64;
+            if (r < BM) load_lds16(as_rsrc, raw0 + r * 16, (r + l) * P.ldas, g * 16);
+            else if (r < BM + BN) load_lds16(ws_rsrc, raw0 + r * 16, (r - BM + l) * P.ldws, g * 16);
+        }
     };
-    auto scl_put = [&]() {
+    auto put_scales = [&]() {
         const int l = hidden_lane();
-        if (has_rows) scl[s_at + l] = bytes4x4(raw[s_at + l]);
+#pragma unroll
+        for (int i = 0; i < SC_LD; i++) {
+            const int r = (gw + 4 * i) * 64;
+            if (r < BM + BN) scl[r + l] = bytes4x4(raw[r + l]);
+        }
     };
 
     f32x4 acc[FM][FN];
@@ -608,56 +621,66 @@ __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const
     for (int i = 0; i < FM; i++)
 #pragma unroll
         for (int j = 0; j < FN; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    i32x8 a8[FM];                /* e4m3: 128 columns */
-    u32x4 a[2][FM], w[KS][FN];   /* e2m1: two times 128 */
+    u32x4 a[2][FM], w[KS][FN];   /* e4m3: A's two halves of a row; e2m1: 128 columns each */
     int sa[FM], sw[FN];
-    /* rows 16 apart are stored alike, chunk 4 + lg is chunk lg XOR 4 */
-    auto frags = [&](const uint8_t *stage) {
-        const int l = hidden_lane(), r = l & 15, c = l >> 4;
-        const int pa = wm * TWM * 128 + r * 128 + ((c ^ (r >> 1)) << 4);
-        const int pw = A_BYTES + wn * TWN * WROW + r * WROW + ((c ^ (F8 ? (r >> 1) & 3 : r >> 1)) << 4);
+    /* fragments of step kt, loads of later steps spread over the reads (either
+     * alone takes most of a phase). Rows 16 apart are stored alike, chunk 4 +
+     * lg is chunk lg XOR 4. */
+    auto frags = [&](int kt, auto &&load, auto loads) {
+        const int l = hidden_lane(), r = l & 15, c = ((l >> 4) ^ (r >> 1)) << 4;
+        const int pa = (kt & 1) * A_BYTES + wm * TWM * 128 + r * 128 + c;
+        const int pw = 2 * A_BYTES + ((F8 ? kt >> 1 : kt) & 1) * W_BYTES + wn * TWN * 128 + r * 128 + (F8 && (kt & 1) ? c ^ 64 : c);
+        constexpr int LOADS = decltype(loads)::value, AR = 2 * FM, READS = AR + KS * FN;
+        int at = 0;
 #pragma unroll
-        for (int i = 0; i < FM; i++) {
-            const u32x4 x = *(const u32x4 *)(stage + pa + i * 2048), y = *(const u32x4 *)(stage + (pa ^ 64) + i * 2048);
-            if constexpr (F8) {
-                a8[i] = (i32x8){(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-            } else {
-                a[0][i] = x;
-                a[1][i] = y;
+        for (int i = 0; i < READS; i++) {
+            if (i * LOADS / READS == at && at < LOADS) {
+                __builtin_amdgcn_sched_barrier(0);
+                load(l, at++);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if (i < AR) a[i / FM][i % FM] = *(const u32x4 *)(lds + (i < FM ? pa : pa ^ 64) + (i % FM) * 2048);
+            else w[(i - AR) / FN][(i - AR) % FN] = *(const u32x4 *)(lds + (i - AR < FN ? pw : pw ^ 64) + ((i - AR) % FN) * 2048);
         }
-#pragma unroll
-        for (int h = 0; h < KS; h++)
-#pragma unroll
-            for (int j = 0; j < FN; j++) w[h][j] = *(const u32x4 *)(stage + (h ? pw ^ 64 : pw) + j * 16 * WROW);
     };
-    auto scales = [&]() {
-        const int l = hidden_lane(), at = (l & 15) * 16 + (l >> 4) * 4, pa = wm * TWM * 16 + at, pw = (BM + wn * TWN) * 16 + at;
+    auto scales = [&](bool first) {
+        if (first) {
+            const int l = hidden_lane(), at = (l & 15) * 16 + (l >> 4) * 4, pa = wm * TWM * 16 + at, pw = (BM + wn * TWN) * 16 + at;
 #pragma unroll
-        for (int i = 0; i < FM; i++) sa[i] = *(const int *)((const uint8_t *)scl + pa + i * 256);
+            for (int i = 0; i < FM; i++) sa[i] = *(const int *)((const uint8_t *)scl + pa + i * 256);
 #pragma unroll
-        for (int j = 0; j < FN; j++) sw[j] = *(const int *)((const uint8_t *)scl + pw + j * 256);
+            for (int j = 0; j < FN; j++) sw[j] = *(const int *)((const uint8_t *)scl + pw + j * 256);
+        } else {
+#pragma unroll
+            for (int i = 0; i < FM; i++) sa[i] = (int)((uint32_t)sa[i] >> 8 * KS);
+#pragma unroll
+            for (int j = 0; j < FN; j++) sw[j] = (int)((uint32_t)sw[j] >> 8 * KS);
+        }
     };
-    /* half h of a K step: e2m1, its 128 columns; e4m3, half of the rows' tiles */
-    auto mfmas = [&](auto s_, auto h_, bool there) {
-        constexpr int S = decltype(s_)::value, H = decltype(h_)::value;
+    auto mfmas = [&](bool both) {
         if constexpr (F8) {
 #pragma unroll
-            for (int i = H * FM / 2; i < (H + 1) * FM / 2; i++) {
-                i32x8 hi = a8[i], lo = a8[i];
-                if constexpr (SPLIT) mx_split(a8[i], hi, lo);
+            for (int i = 0; i < FM; i++) {
+                const u32x4 x = a[0][i], y = a[1][i];
+                i32x8 hi = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]}, lo = hi;
+                if constexpr (SPLIT) mx_split(hi, hi, lo);
 #pragma unroll
-                for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma_op<S, AF>(w[0][j], hi, acc[i][j], sw[j], sa[i]);
+                for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma<AF>(w[0][j], hi, acc[i][j], sw[j], sa[i]);
                 if constexpr (SPLIT)
 #pragma unroll
-                    for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma_op<S, AF>(w[0][j], lo, acc[i][j], sw[j], sa[i]);
+                    for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma<AF>(w[0][j], lo, acc[i][j], sw[j], sa[i]);
             }
-        } else if (H == 0 || there) {
+        } else {
 #pragma unroll
-            for (int i = 0; i < FM; i++) {
-                const i32x8 x = {(int)a[H][i][0], (int)a[H][i][1], (int)a[H][i][2], (int)a[H][i][3], 0, 0, 0, 0};
+            for (int h = 0; h < 2; h++) {
+                if (h && !both) break;
 #pragma unroll
-                for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma_op<2 * S + H, AF>(w[H < KS ? H : 0][j], x, acc[i][j], sw[j], sa[i]);
+                for (int i = 0; i < FM; i++) {
+                    const u32x4 x = a[h][i];
+                    const i32x8 x8 = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < FN; j++) acc[i][j] = h ? mx_mfma4<1>(w[KS - 1][j], x8, acc[i][j], sw[j], sa[i]) : mx_mfma4<0>(w[0][j], x8, acc[i][j], sw[j], sa[i]);
+                }
             }
         }
     };
@@ -681,104 +704,105 @@ __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const
         __builtin_amdgcn_sched_barrier(0);
     };
     /* Phases between barriers: group 0 runs L(t), C(t) in phases 2t, 2t + 1,
-     * group 1 in phases 2t + 1, 2t + 2; L reads step t's fragments (stage t %
-     * 2), C runs its matrix instructions. Each group loads one operand:
-     *  - group 0 issues A of step t + 1 in L(t) into the other stage, which
-     *    both groups read before phase 2t, and waits for it at the end of C(t);
-     *  - group 1 issues W of step t + 2 in L(t) into the stage that it has
-     *    just read, behind a barrier in the middle of phase 2t + 1 (group 0,
-     *    which read step t in phase 2t, meets it inside C(t)), and waits for
-     *    it in L(t + 1).
-     * Scales of 512 columns are read in L of the first step of them, and
-     * those of the next 512 written in L of their last step. Past the last
-     * step the loads repeat it into a stage nothing reads again. */
-    auto step0 = [&](auto s_, auto last_, uint8_t *cur, uint8_t *nxt, int kt, int g) {
-        constexpr int S = decltype(s_)::value, LAST = decltype(last_)::value;
-        const bool there = F8 || !LAST || kt * 2 + 1 < P.steps;
-        if constexpr (S == PER - 1) {
-            if (g + 1 < ng) scl_put();
-        }
-        if constexpr (S == 0) scales();
-        frags(cur);
-        dma_a(nxt, min(kt + 1, nk - 1));
-        if constexpr (S == 0) {
-            if (g + 1 < ng) scl_load(g + 1);
-        }
-        WAIT(63, 0);
+     * group 1 in phases 2t + 1, 2t + 2; L reads step t's fragments, C runs its
+     * matrix instructions. Loads are issued in L only (one that waits for the
+     * address path holds up the instructions behind it), each into memory that
+     * was last read in an earlier phase:
+     *  - A's upper half is read by group 0 alone, in phase 2t: group 1 issues
+     *    that of step t + 2 in L(t), phase 2t + 1, and waits for it at the end
+     *    of L(t + 1), one phase before it is read;
+     *  - A's lower half is read by group 1 alone, in phase 2t + 1, W by both:
+     *    group 0 issues in L(t) W's next (e4m3: of the next 256 columns, half
+     *    in either of two steps), waited for at the end of C(t), and A's lower
+     *    half of step t + 1, waited for at the end of L(t + 1).
+     * Loads of a wave complete in order, so a wait names the number of younger
+     * ones. Scales of the next 512 columns: group 1 loads them in the first
+     * step of 512 columns, behind its part of A, and writes them to their place
+     * in the last; both groups read them in the first. Past the end the loads
+     * repeat the last step's, into a stage that nothing reads again. */
+    auto step0 = [&](int kt, auto s_) {
+        constexpr int S = decltype(s_)::value;
+        const int kw = min((F8 ? kt >> 1 : kt) + 1, nw - 1), ka = min(kt + 1, nk - 1);
+        const int wdst = (F8 ? kt >> 1 : kt) + 1;
+        scales(S == 0);
+        frags(kt, [&](int l, int i) {
+            if (i < W_LD) load_w(kw, wdst, F8 ? kt & 1 : 0, l, i);
+            else load_a(1, ka, kt + 1, l, i - W_LD);
+        }, Const<W_LD + A_LD>{});
+        WAIT(W_LD + A_LD, 0);
         barrier();
-        mfmas(s_, Const<0>{}, there);
+        mfmas(2 * kt + 1 < P.steps);
         pin();
-        barrier();   /* group 1's reads of step kt are done */
-        mfmas(s_, Const<1>{}, there);
-        pin();
-        WAIT(0, 0);
+        WAIT(A_LD, 0);
         barrier();
     };
-    auto step1 = [&](auto s_, auto last_, uint8_t *cur, int kt, int g) {
-        constexpr int S = decltype(s_)::value, LAST = decltype(last_)::value;
-        const bool there = F8 || !LAST || kt * 2 + 1 < P.steps;
-        if constexpr (S == 0) scales();
-        frags(cur);
-        WAIT(0, 0);
-        barrier();   /* every wave of the group has read step kt */
-        dma_w(cur, min(kt + 2, nk - 1));
-        if constexpr (S == 0) {
-            if (g + 1 < ng) scl_load(g + 1);
-        }
+    auto step1 = [&](int kt, auto s_) {
+        constexpr int S = decltype(s_)::value;
         if constexpr (S == PER - 1) {
-            if (g + 1 < ng) scl_put();
-            WAIT(63, 0);
+            if constexpr (PER == 2) WAIT(0, 15);
+            put_scales();
         }
+        scales(S == 0);
+        const int ka = min(kt + 2, nk - 1);
+        frags(kt, [&](int l, int i) { load_a(0, ka, kt, l, i); }, Const<A_LD>{});
+        if constexpr (S == 0) load_scales(min(kt / PER + 1, ng - 1));
+        WAIT(A_LD + (S == 0 ? SC_LD : 0), 0);
         barrier();
-        mfmas(s_, Const<0>{}, there);
-        mfmas(s_, Const<1>{}, there);
+        mfmas(2 * kt + 1 < P.steps);
         pin();
         if (kt + 1 < nk) barrier();
     };
-    scl_load(0);
+    {
+        const int l = hidden_lane(), k1 = min(1, nk - 1);
+        if (grp) {
+#pragma unroll
+            for (int i = 0; i < A_LD; i++) load_a(0, 0, 0, l, i);
+#pragma unroll
+            for (int i = 0; i < A_LD; i++) load_a(0, k1, 1, l, i);
+            load_scales(0);
+            WAIT(0, 0);
+            put_scales();
+            WAIT(63, 0);
+        } else {
+#pragma unroll
+            for (int s = 0; s < (F8 ? 2 : 1); s++)
+#pragma unroll
+                for (int i = 0; i < W_LD; i++) load_w(0, 0, s, l, i);
+#pragma unroll
+            for (int i = 0; i < A_LD; i++) load_a(1, 0, 0, l, i);
+            WAIT(0, 0);
+        }
+    }
+    barrier();
+    const int whole = nk / PER * PER;
     if (grp) {
-        dma_w(lds0, 0);
-        WAIT(0, 0);
-        scl_put();
-        WAIT(0, 0);
         barrier();
-        dma_w(lds1, min(1, nk - 1));
-        barrier();
-        const int whole = P.steps / 4;
-        for (int g = 0; g < whole; g++) {
-            step1(Const<0>{}, Const<0>{}, lds0, g * PER, g);
-            step1(Const<1>{}, Const<0>{}, lds1, g * PER + 1, g);
+        for (int kt = 0; kt < whole; kt += PER) {
+            step1(kt, Const<0>{});
+            step1(kt + 1, Const<1>{});
             if constexpr (PER == 4) {
-                step1(Const<2>{}, Const<0>{}, lds0, g * PER + 2, g);
-                step1(Const<3>{}, Const<0>{}, lds1, g * PER + 3, g);
+                step1(kt + 2, Const<2>{});
+                step1(kt + 3, Const<3>{});
             }
         }
-        const int kt = whole * PER;
-        if (kt < nk) step1(Const<0>{}, Const<1>{}, lds0, kt, whole);
-        if (kt + 1 < nk) step1(Const<1>{}, Const<1>{}, lds1, kt + 1, whole);
+        if (whole < nk) step1(whole, Const<0>{});
         if constexpr (PER == 4) {
-            if (kt + 2 < nk) step1(Const<2>{}, Const<1>{}, lds0, kt + 2, whole);
+            if (whole + 1 < nk) step1(whole + 1, Const<1>{});
+            if (whole + 2 < nk) step1(whole + 2, Const<2>{});
         }
     } else {
-        dma_a(lds0, 0);
-        WAIT(0, 0);
-        scl_put();
-        WAIT(0, 0);
-        barrier();
-        const int whole = P.steps / 4;
-        for (int g = 0; g < whole; g++) {
-            step0(Const<0>{}, Const<0>{}, lds0, lds1, g * PER, g);
-            step0(Const<1>{}, Const<0>{}, lds1, lds0, g * PER + 1, g);
+        for (int kt = 0; kt < whole; kt += PER) {
+            step0(kt, Const<0>{});
+            step0(kt + 1, Const<1>{});
             if constexpr (PER == 4) {
-                step0(Const<2>{}, Const<0>{}, lds0, lds1, g * PER + 2, g);
-                step0(Const<3>{}, Const<0>{}, lds1, lds0, g * PER + 3, g);
+                step0(kt + 2, Const<2>{});
+                step0(kt + 3, Const<3>{});
             }
         }
-        const int kt = whole * PER;
-        if (kt < nk) step0(Const<0>{}, Const<1>{}, lds0, lds1, kt, whole);
-        if (kt + 1 < nk) step0(Const<1>{}, Const<1>{}, lds1, lds0, kt + 1, whole);
+        if (whole < nk) step0(whole, Const<0>{});
         if constexpr (PER == 4) {
-            if (kt + 2 < nk) step0(Const<2>{}, Const<1>{}, lds0, lds1, kt + 2, whole);
+            if (whole + 1 < nk) step0(whole + 1, Const<1>{});
+            if (whole + 2 < nk) step0(whole + 2, Const<2>{});
         }
     }
     WAIT(0, 0);   /* no load outstanding at exit */
@@ -788,8 +812,8 @@ __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const
      * or 64 bytes) is written by neighbouring lanes: 8-byte stores of 16 rows
      * each took 10 us more of 4096 x 4096 x 2560. */
     const bool full = m0 + BM <= P.M && n0 + BN <= P.N;
-    uint8_t *const st = (grp ? lds1 : lds0) + gw * 8192;
-    static_assert(STAGE >= 4 * 8192, "a wave's part of a stage");
+    uint8_t *const st = lds + wave * 8192;
+    static_assert(sizeof(lds) >= 8 * 8192, "a wave's part");
     if (full && P.epi == IRIS_EPI_BF16 && rows16_ok(P.out, P.ldo)) {
         __syncthreads();   /* every wave is done with the stages */
 #pragma unroll
