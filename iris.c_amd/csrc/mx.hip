@@ -13,6 +13,8 @@
  */
 #include "iris_internal.h"
 
+#include <mutex>
+
 namespace {
 
 constexpr int NT = 256;
@@ -278,7 +280,23 @@ struct MxGemm {
     int M, N, steps, ldo, epi;
     uint8_t *oq, *os;      /* SWIGLU: microscaled output, NULL: bf16 into out */
     int ldoq, ldos, ofmt;
+    /* blocks: tiles_m x tiles_n of them for each of `chunks` ranges of per_chunk
+     * K steps; with more than one, out is f32 [chunk][M][N] partial sums */
+    int tiles_m, tiles_n, chunks, per_chunk;
 };
+
+/* The K range of chunk c: operands from its first step on, partial sums out.
+ * per_chunk is a multiple of 4 steps, 16 scale bytes. */
+template <int AF> __device__ __forceinline__ void mx_chunk(MxGemm &P, int c) {
+    if (P.chunks == 1) return;
+    const int k0 = c * P.per_chunk;
+    P.aq += (size_t)k0 * (AF == IRIS_MX_FP8 ? 128 : 64);
+    P.wq += (size_t)k0 * 64;
+    P.as += (size_t)k0 * 4;
+    P.ws += (size_t)k0 * 4;
+    P.steps = min(P.per_chunk, P.steps - k0);
+    P.out = (float *)P.out + (size_t)c * P.M * P.N;
+}
 
 /* The instruction adds its products in groups of 8 neighbouring columns and
  * keeps, of a group, bits down to 2^-13 of the largest product's power of two
@@ -301,14 +319,15 @@ __device__ __forceinline__ f32x4 mx_mfma4(const u32x4 &w, const i32x8 &a, const 
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, a, c, 4, 4, OP, sw, OP, sa);
 }
 
-/* e4m3 codes of magnitude 2 and more (bit 6 set), and the others */
-__device__ __forceinline__ void mx_split(const i32x8 &a, i32x8 &hi, i32x8 &lo) {
+/* the e4m3 codes of magnitude 2 and more (bit 6 set), or the others */
+template <bool BIG> __device__ __forceinline__ i32x8 mx_part(const i32x8 &a) {
+    i32x8 r;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const uint32_t x = (uint32_t)a[i], big = ((x >> 6) & 0x01010101u) * 255u;
-        hi[i] = (int)(x & big);
-        lo[i] = (int)(x & ~big);
+        r[i] = (int)(BIG ? x & big : x & ~big);
     }
+    return r;
 }
 
 /* one lane's 4 columns n .. n + 3 of row m through the plain epilogues */
@@ -406,89 +425,153 @@ __device__ __forceinline__ void mx_store_swiglu(const MxGemm &P, int m, int n, c
         }
 }
 
-/* A block's 8 waves share 16 FM rows of A and 16 FN of W and take every
- * eighth K step of 128 each, fragments straight from global memory; their sums
- * are added in wave order through LDS. */
-template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm_direct_kernel(const MxGemm P) {
-    __shared__ f32x4 part[8][64];
-    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4, wave = tid >> 6;
-    const int tiles_n = (P.N + 16 * FN - 1) / (16 * FN);
-    const int m0 = (int)(blockIdx.x / tiles_n) * 16 * FM, n0 = (int)(blockIdx.x % tiles_n) * 16 * FN;
+/* ---- product of few rows ----
+ * Bound by W's bytes, not by the matrix instructions. A block's 8 waves share
+ * 16 FM rows of A and 16 FN of W and take consecutive parts of K, fragments
+ * straight from global memory, U steps of 128 in flight per wave: 16 rows of W
+ * and one of A keep 8 waves x 4 KiB in flight. The waves' sums are added in
+ * wave order through LDS. */
+template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm_rows_kernel(MxGemm P) {
+    constexpr int U = FM * FN == 1 ? 4 : FM == 1 ? 3 : 2;
+    extern __shared__ f32x4 part[];   /* [8 waves][FM * FN tiles][64 lanes] */
+    const int tiles = P.tiles_m * P.tiles_n;
+    const int chunk = (int)blockIdx.x / tiles, t = (int)blockIdx.x - chunk * tiles;
+    mx_chunk<AF>(P, chunk);
+    const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m0 = t / P.tiles_n * 16 * FM, n0 = t % P.tiles_n * 16 * FN;
     const uint8_t *ap[FM], *sap[FM], *wp[FN], *swp[FN];
 #pragma unroll
     for (int i = 0; i < FM; i++) {
         const size_t m = min(m0 + 16 * i + lr, P.M - 1);   /* rows past the end repeat the last; not stored */
         ap[i] = P.aq + m * P.lda + 16 * lg;
-        sap[i] = P.as + m * P.ldas + lg;
+        sap[i] = P.as + m * P.ldas;
     }
 #pragma unroll
     for (int j = 0; j < FN; j++) {
         const size_t n = min(n0 + 16 * j + lr, P.N - 1);
         wp[j] = P.wq + n * P.ldw + 16 * lg;
-        swp[j] = P.ws + n * P.ldws + lg;
+        swp[j] = P.ws + n * P.ldws;
     }
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; i++)
 #pragma unroll
         for (int j = 0; j < FN; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = wave; k < P.steps; k += 8) {
-        u32x4 w[FN];
-        i32x8 a[FM];
-        int sw[FN], sa[FM];
+    const int per = (P.steps + 7) / 8, k1 = min((wave + 1) * per, P.steps);
+    for (int k0 = wave * per; k0 < k1; k0 += U) {
+        u32x4 w[U][FN], a[U][FM][2];
+        uint32_t sw[U][FN], sa[U][FM];
 #pragma unroll
-        for (int j = 0; j < FN; j++) {
-            w[j] = *(const u32x4 *)(wp[j] + (size_t)k * 64);
-            sw[j] = swp[j][k * 4];
-        }
+        for (int u = 0; u < U; u++) {
+            const int k = min(k0 + u, k1 - 1);
 #pragma unroll
-        for (int i = 0; i < FM; i++) {
-            sa[i] = sap[i][k * 4];
-            if constexpr (AF == IRIS_MX_FP8) {
-                const u32x4 lo = *(const u32x4 *)(ap[i] + (size_t)k * 128), hi = *(const u32x4 *)(ap[i] + (size_t)k * 128 + 64);
-                a[i] = (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-            } else {
-                const u32x4 lo = *(const u32x4 *)(ap[i] + (size_t)k * 64);
-                a[i] = (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
+            for (int j = 0; j < FN; j++) {
+                w[u][j] = *(const u32x4 *)(wp[j] + (size_t)k * 64);
+                sw[u][j] = *(const uint32_t *)(swp[j] + k * 4);
+            }
+#pragma unroll
+            for (int i = 0; i < FM; i++) {
+                const uint8_t *x = ap[i] + (size_t)k * (AF == IRIS_MX_FP8 ? 128 : 64);
+                a[u][i][0] = *(const u32x4 *)x;
+                a[u][i][1] = AF == IRIS_MX_FP8 ? *(const u32x4 *)(x + 64) : (u32x4){0, 0, 0, 0};
+                sa[u][i] = *(const uint32_t *)(sap[i] + k * 4);
             }
         }
 #pragma unroll
-        for (int i = 0; i < FM; i++) {
-            i32x8 hi = a[i], lo = a[i];
-            if constexpr (AF == IRIS_MX_FP8) mx_split(a[i], hi, lo);
+        for (int u = 0; u < U; u++) {
+            if (k0 + u >= k1) break;
 #pragma unroll
-            for (int j = 0; j < FN; j++) {
-                acc[i][j] = mx_mfma<AF>(w[j], hi, acc[i][j], sw[j], sa[i]);
-                if constexpr (AF == IRIS_MX_FP8) acc[i][j] = mx_mfma<AF>(w[j], lo, acc[i][j], sw[j], sa[i]);
+            for (int i = 0; i < FM; i++) {
+                const u32x4 x = a[u][i][0], y = a[u][i][1];
+                const i32x8 x8 = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+                const i32x8 hi = AF == IRIS_MX_FP8 ? mx_part<true>(x8) : x8, lo = mx_part<false>(x8);
+                const int s = (int)(sa[u][i] >> 8 * lg);
+#pragma unroll
+                for (int j = 0; j < FN; j++) {
+                    const int r = (int)(sw[u][j] >> 8 * lg);
+                    acc[i][j] = mx_mfma<AF>(w[u][j], hi, acc[i][j], r, s);
+                    if constexpr (AF == IRIS_MX_FP8) acc[i][j] = mx_mfma<AF>(w[u][j], lo, acc[i][j], r, s);
+                }
             }
         }
     }
-    /* wave i % 8 sums tile i of a row of tiles */
-    const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
-    f32x4 mine[FM][FN];   /* only wave 0 keeps the sums */
 #pragma unroll
     for (int i = 0; i < FM; i++)
 #pragma unroll
-        for (int j = 0; j < FN; j++) {
-            __syncthreads();
-            part[wave][lane] = acc[i][j];
-            __syncthreads();
-            f32x4 s = part[0][lane];
+        for (int j = 0; j < FN; j++) part[(wave * FM * FN + i * FN + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    auto sum = [&](int i, int j) {
+        f32x4 s = part[(i * FN + j) * 64 + lane];
 #pragma unroll
-            for (int w = 1; w < 8; w++) s += part[w][lane];
-            mine[i][j] = s;
-        }
-    if (wave) return;
-#pragma unroll
-    for (int i = 0; i < FM; i++) {
-        const int m = m0 + 16 * i + lr;
-        if (FN == 4 && P.epi == IRIS_EPI_SWIGLU) {
-            if constexpr (FN == 4) mx_store_swiglu(P, m, n0, mine[i][0], mine[i][1], mine[i][2], mine[i][3], aligned);
-        } else if (m < P.M) {
-#pragma unroll
-            for (int j = 0; j < FN; j++) mx_store4(P, m, n0 + 16 * j + 4 * lg, mine[i][j], aligned);
+        for (int w = 1; w < 8; w++) s += part[(w * FM * FN + i * FN + j) * 64 + lane];
+        return s;
+    };
+    const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
+    if constexpr (FN == 4) {
+        if (P.epi == IRIS_EPI_SWIGLU) {
+            if (wave < FM) mx_store_swiglu(P, m0 + 16 * wave + lr, n0, sum(wave, 0), sum(wave, 1), sum(wave, 2), sum(wave, 3), aligned);
+            return;
         }
     }
+    for (int q = wave; q < FM * FN; q += 8) {
+        const int m = m0 + 16 * (q / FN) + lr;
+        const f32x4 s = sum(q / FN, q % FN);
+        if (m < P.M) mx_store4(P, m, n0 + 16 * (q % FN) + 4 * lg, s, aligned);
+    }
+}
+
+/* ---- sums of a split product ----
+ * One lane per 8 output columns: the chunks' partial sums in order, then the
+ * epilogue. */
+__global__ __launch_bounds__(NT) void mx_reduce_kernel(const MxGemm P, const float *part, uint32_t n, uint32_t cpr) {
+    const uint32_t i = blockIdx.x * NT + threadIdx.x;
+    if (i >= n) return;
+    const uint32_t m = i / cpr;
+    const int c = (int)(i - m * cpr) * 8;
+    const bool swiglu = P.epi == IRIS_EPI_SWIGLU;
+    const size_t stride = (size_t)P.M * P.N;
+    const bool vec = (P.N & 3) == 0 && ((uintptr_t)part & 15) == 0;
+    auto sum8 = [&](int col) {
+        Row8 s = load8<false>(part + (size_t)m * P.N, col, P.N, vec);
+        for (int k = 1; k < P.chunks; k++) {
+            const Row8 x = load8<false>(part + k * stride + (size_t)m * P.N, col, P.N, vec);
+#pragma unroll
+            for (int j = 0; j < 8; j++) s.v[j] += x.v[j];
+        }
+        return s;
+    };
+    if (!swiglu) {
+        const Row8 s = sum8(c);
+        const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
+        mx_store4(P, (int)m, c, (f32x4){s.v[0], s.v[1], s.v[2], s.v[3]}, aligned);
+        if (c + 4 < P.N) mx_store4(P, (int)m, c + 4, (f32x4){s.v[4], s.v[5], s.v[6], s.v[7]}, aligned);
+        return;
+    }
+    /* columns c .. c + 7 of the output: gate and up columns of one 64-column group */
+    Row8 y;
+    if (c < P.N / 2) {
+        const Row8 g = sum8((c >> 5) * 64 + (c & 31)), u = sum8((c >> 5) * 64 + 32 + (c & 31));
+#pragma unroll
+        for (int j = 0; j < 8; j++) y.v[j] = g.v[j] / (1.0f + expf(-g.v[j])) * u.v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) y.v[j] = 0.0f;   /* a microscaled row's padding */
+    }
+    if (P.oq) {
+        uint8_t *q = P.oq + (size_t)m * P.ldoq, *sc = P.os + (size_t)m * P.ldos;
+        if (P.ofmt == IRIS_MX_FP8) mx_put8<IRIS_MX_FP8>(q, sc, c, y);
+        else mx_put8<IRIS_MX_FP4>(q, sc, c, y);
+        return;
+    }
+    uint16_t *o = (uint16_t *)P.out + (size_t)m * P.ldo + c;
+    u32x4 b;
+#pragma unroll
+    for (int j = 0; j < 4; j++) b[j] = (uint32_t)f2bf_hw(y.v[2 * j]) | (uint32_t)f2bf_hw(y.v[2 * j + 1]) << 16;
+    if ((P.ldo & 7) == 0 && ((uintptr_t)P.out & 15) == 0) *(u32x4 *)o = b;
+    else
+#pragma unroll
+        for (int j = 0; j < 8; j++) o[j] = (uint16_t)(b[j >> 1] >> (16 * (j & 1)));
 }
 
 /* ---- product on LDS tiles ----
@@ -510,9 +593,6 @@ constexpr int waitcnt_imm(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 1
 typedef __attribute__((address_space(3))) void lds_void;
 constexpr int GROUP_M = 8;
 
-struct MxTiles {
-    int tiles_m, tiles_n, per_xcd;
-};
 
 /* 64 lanes' 16 bytes from a buffer to LDS, one after the other from place at on
  * (rows past the buffer's end: zeros). Not the builtin: before reads of one
@@ -545,7 +625,7 @@ template <int V> struct Const {
 };
 
 template <int AF, bool SPLIT, int BM, int BN>
-__global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const MxTiles T) {
+__global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(MxGemm P) {
     constexpr bool F8 = AF == IRIS_MX_FP8;
     constexpr int KS = F8 ? 1 : 2, PER = 4 / KS;   /* 128 columns per step, steps per 512 columns */
     constexpr int TWM = BM / 4, TWN = BN / 2, FM = TWM / 16, FN = TWN / 16;
@@ -555,27 +635,30 @@ __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * (A_BYTES + W_BYTES)];
     __shared__ u32x4 raw[BM + BN];
     __shared__ u32x4 scl[BM + BN];
-    const int L = (int)(blockIdx.x & 7) * T.per_xcd + (int)(blockIdx.x >> 3);
-    if (L >= T.tiles_m * T.tiles_n) return;
-    const int first_m = L / (GROUP_M * T.tiles_n) * GROUP_M, gsz = min(T.tiles_m - first_m, GROUP_M);
-    const int tg = L - first_m * T.tiles_n, tn = tg / gsz;
+    const int tiles = P.tiles_m * P.tiles_n, per_xcd = (tiles * P.chunks + 7) / 8;
+    const int L = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if (L >= tiles * P.chunks) return;
+    const int chunk = L / tiles, t = L - chunk * tiles;
+    const int first_m = t / (GROUP_M * P.tiles_n) * GROUP_M, gsz = min(P.tiles_m - first_m, GROUP_M);
+    const int tg = t - first_m * P.tiles_n, tn = tg / gsz;
     const int m0 = (first_m + tg - tn * gsz) * BM, n0 = tn * BN;
+    const int off = chunk * P.per_chunk;   /* the buffers below end where the rows do */
+    mx_chunk<AF>(P, chunk);
 
-    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = wave >> 2, gw = wave & 3;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = wave >> 2, gw = wave & 3;
     const int wm = wave >> 1, wn = wave & 1;
 
     /* rows past the end read as zeros */
-    const u32x4 a_rsrc = buffer_of(P.aq + (size_t)m0 * P.lda, min(BM, P.M - m0) * P.lda);
-    const u32x4 w_rsrc = buffer_of(P.wq + (size_t)n0 * P.ldw, min(BN, P.N - n0) * P.ldw);
-    const u32x4 as_rsrc = buffer_of(P.as + (size_t)m0 * P.ldas, min(BM, P.M - m0) * P.ldas);
-    const u32x4 ws_rsrc = buffer_of(P.ws + (size_t)n0 * P.ldws, min(BN, P.N - n0) * P.ldws);
+    const u32x4 a_rsrc = buffer_of(P.aq + (size_t)m0 * P.lda, min(BM, P.M - m0) * P.lda - off * (F8 ? 128 : 64));
+    const u32x4 w_rsrc = buffer_of(P.wq + (size_t)n0 * P.ldw, min(BN, P.N - n0) * P.ldw - off * 64);
+    const u32x4 as_rsrc = buffer_of(P.as + (size_t)m0 * P.ldas, min(BM, P.M - m0) * P.ldas - off * 4);
+    const u32x4 ws_rsrc = buffer_of(P.ws + (size_t)n0 * P.ldws, min(BN, P.N - n0) * P.ldws - off * 4);
     const int nk = (P.steps + KS - 1) / KS, nw = (P.steps + 1) / 2, ng = (P.steps + 3) / 4;
     const uint32_t at0 = lds_at(lds), raw0 = lds_at(raw);
     auto hidden_lane = [&]() {   /* places are computed anew in each step: registers are short */
-        int l = lane;
-        asm volatile("" : "+v"(l));
-        return l;
+        int zero = 0;
+        asm volatile("" : "+s"(zero));
+        return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, (unsigned)zero));
     };
     /* A load covers 8 rows: lane l row l / 8, place l % 8, chunk place ^ (row /
      * 2 % 8), which depends on the load by its parity. Of 256 columns that the
@@ -662,13 +745,17 @@ __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const
 #pragma unroll
             for (int i = 0; i < FM; i++) {
                 const u32x4 x = a[0][i], y = a[1][i];
-                i32x8 hi = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]}, lo = hi;
-                if constexpr (SPLIT) mx_split(hi, hi, lo);
+                const i32x8 x8 = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+                const i32x8 hi = SPLIT ? mx_part<true>(x8) : x8;
 #pragma unroll
                 for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma<AF>(w[0][j], hi, acc[i][j], sw[j], sa[i]);
-                if constexpr (SPLIT)
+                if constexpr (SPLIT) {
+                    __builtin_amdgcn_sched_barrier(0);   /* one part in registers at a time */
+                    const i32x8 lo = mx_part<false>(x8);
 #pragma unroll
                     for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma<AF>(w[0][j], lo, acc[i][j], sw[j], sa[i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         } else {
 #pragma unroll
@@ -807,6 +894,7 @@ __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const
     }
     WAIT(0, 0);   /* no load outstanding at exit */
 #undef WAIT
+    const int lane = hidden_lane(), lr = lane & 15, lg = lane >> 4;
     /* Whole tiles of 16-bit or microscaled output leave through LDS, two of a
      * wave's 16-row tiles at a time, so that a row's part of a wave (256, 128
      * or 64 bytes) is written by neighbouring lanes: 8-byte stores of 16 rows
@@ -836,8 +924,8 @@ __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const
             uint16_t *const out = (uint16_t *)P.out + (size_t)(m0 + wm * TWM + ip * 16) * P.ldo + n0 + wn * TWN;
             constexpr int CPR = FN * 2;
 #pragma unroll
-            for (int c = lane; c < 32 * CPR; c += 64) {
-                const int row = c / CPR, ch = c % CPR;
+            for (int k = 0; k < 32 * CPR / 64; k++) {
+                const int c = k * 64 + lane, row = c / CPR, ch = c % CPR;
                 *(u32x4 *)(out + (size_t)row * P.ldo + ch * 8) = *(const u32x4 *)(st + row * (TWN * 2) + ((ch ^ (row & (CPR - 1))) << 4));
             }
         }
@@ -864,8 +952,8 @@ __global__ __launch_bounds__(512) void mx_gemm_tile_kernel(const MxGemm P, const
             uint16_t *const out = (uint16_t *)P.out + (size_t)(m0 + wm * TWM + ip * 16) * P.ldo + (n0 + wn * TWN) / 2;
             constexpr int CPR = FN;
 #pragma unroll
-            for (int c = lane; c < 32 * CPR; c += 64) {
-                const int row = c / CPR, ch = c % CPR;
+            for (int k = 0; k < 32 * CPR / 64; k++) {
+                const int c = k * 64 + lane, row = c / CPR, ch = c % CPR;
                 *(u32x4 *)(out + (size_t)row * P.ldo + ch * 8) = *(const u32x4 *)(st + row * TWN + ((ch ^ (row & (CPR - 1))) << 4));
             }
         }
@@ -1025,6 +1113,69 @@ extern "C" int iris_hip_mx_rmsnorm(const iris_mx_norm_t *a) {
     return iris_launch_check("mx_rmsnorm_kernel");
 }
 
+/* ---- which kernel, and whether K is split ---- */
+namespace {
+enum { MX_ROWS, MX_TILE128, MX_TILE256 };
+struct MxPlan {
+    int kind, fm, fn, tiles_m, tiles_n, chunks, per_chunk;
+};
+
+template <int AF, int FM, int FN> int launch_rows_of(const MxGemm &P, unsigned blocks) {
+    constexpr int smem = 8 * FM * FN * 1024;
+    static std::once_flag once;
+    static hipError_t attr = hipSuccess;
+    std::call_once(once, [] {
+        attr = hipFuncSetAttribute((const void *)mx_gemm_rows_kernel<AF, FM, FN>, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+    });
+    if (iris_check(attr, "mx_gemm_rows smem attribute")) return -1;
+    IRIS_LAUNCH((mx_gemm_rows_kernel<AF, FM, FN>), dim3(blocks), dim3(512), smem, iris_stream(), P);
+    return 0;
+}
+template <int AF> int launch_rows(const MxGemm &P, const MxPlan &plan, unsigned blocks) {
+    if (plan.fn == 1) return launch_rows_of<AF, 1, 1>(P, blocks);
+    if (plan.fm == 1) return launch_rows_of<AF, 1, 4>(P, blocks);
+    if (plan.fm == 2) return launch_rows_of<AF, 2, 4>(P, blocks);
+    return launch_rows_of<AF, 4, 4>(P, blocks);
+}
+
+MxPlan mx_plan(const iris_mx_gemm_t &p, int steps, size_t ws_bytes) {
+    const int cus = iris_cu_count();
+    MxPlan q;
+    /* tile loads reach rows by 32-bit offsets */
+    long long ld = p.A.ld_q;
+    for (int v : {p.W.ld_q, p.A.ld_s, p.W.ld_s}) ld = v > ld ? v : ld;
+    const bool far = ld * 256 > 0x7fffffffLL;
+    int bm, bn;
+    if (p.M <= 64 || far) {
+        q.kind = MX_ROWS;
+        q.fm = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+        q.fn = q.fm == 1 && p.epi != IRIS_EPI_SWIGLU ? 1 : 4;
+        bm = 16 * q.fm;
+        bn = 16 * q.fn;
+    } else {
+        const long long t256 = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
+        q.kind = t256 * 2 > cus ? MX_TILE256 : MX_TILE128;
+        bm = bn = q.kind == MX_TILE256 ? 256 : 128;
+    }
+    q.tiles_m = (p.M + bm - 1) / bm;
+    q.tiles_n = (p.N + bn - 1) / bn;
+    q.chunks = 1;
+    q.per_chunk = steps;
+    const long long tiles = (long long)q.tiles_m * q.tiles_n;
+    if (ws_bytes && tiles * 2 <= cus && steps >= 16 && (size_t)p.M * ((p.N + 127) / 128 * 16) < (1u << 31)) {
+        long long c = cus / tiles;
+        const long long most = (long long)(ws_bytes / ((size_t)p.M * p.N * 4));
+        if (c > most) c = most;
+        if (c > steps / 8) c = steps / 8;
+        if (c > 1) {
+            q.per_chunk = (int)((steps + c - 1) / c + 3) / 4 * 4;
+            q.chunks = (steps + q.per_chunk - 1) / q.per_chunk;
+        }
+    }
+    return q;
+}
+}  // namespace
+
 extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_bytes) {
     if (!p) return iris_set_error("mx_gemm: null problem");
     if (p->M <= 0 || p->N <= 0) return 0;
@@ -1041,8 +1192,6 @@ extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_by
     if (mx ? check_mx("mx_gemm output", p->mx_out, nout) : !p->out ? iris_set_error("mx_gemm: null output") : 0) return -1;
     if (!mx && p->ldo < nout) return iris_set_error("mx_gemm: output row stride %d of %d columns", p->ldo, nout);
     if (!iris_hip_available()) return -1;
-    (void)ws;
-    (void)ws_bytes;
     MxGemm P;
     P.aq = p->A.q; P.as = p->A.s; P.lda = p->A.ld_q; P.ldas = p->A.ld_s;
     P.wq = p->W.q; P.ws = p->W.s; P.ldw = p->W.ld_q; P.ldws = p->W.ld_s;
@@ -1050,30 +1199,40 @@ extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_by
     P.steps = pad_to(p->K, 128) / 128;
     P.oq = mx ? p->mx_out.q : nullptr; P.os = p->mx_out.s;
     P.ldoq = p->mx_out.ld_q; P.ldos = p->mx_out.ld_s; P.ofmt = p->mx_out.fmt;
-    const bool far = (long long)(p->A.ld_q > p->W.ld_q ? p->A.ld_q : p->W.ld_q) * 256 > 0x7fffffffLL;
-    if (p->M > 128 && !far) {
-        MxTiles T;
-        T.tiles_m = (p->M + 255) / 256;
-        T.tiles_n = (p->N + 255) / 256;
-        const long long total = (long long)T.tiles_m * T.tiles_n;
-        if (total > 0x7fffffff / 2) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
-        T.per_xcd = (int)((total + 7) / 8);
-        const bool exact = p->epi != IRIS_EPI_BF16 && !swiglu;
-        const dim3 grid(8 * T.per_xcd);
-        if (p->A.fmt == IRIS_MX_FP4)
-            IRIS_LAUNCH((mx_gemm_tile_kernel<IRIS_MX_FP4, false, 256, 256>), grid, dim3(512), 0, iris_stream(), P, T);
-        else if (exact)
-            IRIS_LAUNCH((mx_gemm_tile_kernel<IRIS_MX_FP8, true, 256, 256>), grid, dim3(512), 0, iris_stream(), P, T);
-        else
-            IRIS_LAUNCH((mx_gemm_tile_kernel<IRIS_MX_FP8, false, 256, 256>), grid, dim3(512), 0, iris_stream(), P, T);
-        return iris_launch_check("mx_gemm_tile_kernel");
+    const MxPlan plan = mx_plan(*p, P.steps, ((uintptr_t)ws & 15) || !ws ? 0 : ws_bytes);
+    P.tiles_m = plan.tiles_m; P.tiles_n = plan.tiles_n; P.chunks = plan.chunks; P.per_chunk = plan.per_chunk;
+    const long long blocks = (long long)plan.tiles_m * plan.tiles_n * plan.chunks;
+    if (blocks > 0x7fffffff / 2) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
+    MxGemm R = P;
+    if (plan.chunks > 1) {
+        P.out = ws; P.ldo = p->N; P.vec = nullptr; P.epi = IRIS_EPI_F32; P.oq = nullptr;
     }
-    constexpr int FM = 4, FN = 4;
-    const long long tiles = (long long)((p->M + 16 * FM - 1) / (16 * FM)) * ((p->N + 16 * FN - 1) / (16 * FN));
-    if (tiles > 0x7fffffffLL) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
-    if (p->A.fmt == IRIS_MX_FP8)
-        IRIS_LAUNCH((mx_gemm_direct_kernel<IRIS_MX_FP8, FM, FN>), dim3((unsigned)tiles), dim3(512), 0, iris_stream(), P);
-    else
-        IRIS_LAUNCH((mx_gemm_direct_kernel<IRIS_MX_FP4, FM, FN>), dim3((unsigned)tiles), dim3(512), 0, iris_stream(), P);
-    return iris_launch_check("mx_gemm_direct_kernel");
+    const bool f8 = p->A.fmt == IRIS_MX_FP8;
+    if (plan.kind == MX_ROWS) {
+        if (f8 ? launch_rows<IRIS_MX_FP8>(P, plan, (unsigned)blocks) : launch_rows<IRIS_MX_FP4>(P, plan, (unsigned)blocks)) return -1;
+    } else {
+        /* 16- and 8-bit results are rounded 100 times coarser than what the
+         * single instruction loses; f32 results get f32 sums */
+        const bool exact = f8 && !swiglu && p->epi != IRIS_EPI_BF16;
+        const dim3 grid((unsigned)((blocks + 7) / 8 * 8));
+#define MX_T(F, X, T) IRIS_LAUNCH((mx_gemm_tile_kernel<F, X, T, T>), grid, dim3(512), 0, iris_stream(), P)
+        if (plan.kind == MX_TILE256) {
+            if (!f8) MX_T(IRIS_MX_FP4, false, 256);
+            else if (exact) MX_T(IRIS_MX_FP8, true, 256);
+            else MX_T(IRIS_MX_FP8, false, 256);
+        } else {
+            if (!f8) MX_T(IRIS_MX_FP4, false, 128);
+            else if (exact) MX_T(IRIS_MX_FP8, true, 128);
+            else MX_T(IRIS_MX_FP8, false, 128);
+        }
+#undef MX_T
+    }
+    if (iris_launch_check("mx_gemm kernel")) return -1;
+    if (plan.chunks > 1) {
+        const int cols = mx ? pad_to(nout, 128) : nout;
+        const uint32_t cpr = (uint32_t)(cols + 7) / 8, n = (uint32_t)p->M * cpr;
+        IRIS_LAUNCH(mx_reduce_kernel, dim3((n + NT - 1) / NT), dim3(NT), 0, iris_stream(), R, (const float *)ws, n, cpr);
+        return iris_launch_check("mx_reduce_kernel");
+    }
+    return 0;
 }

@@ -344,6 +344,25 @@ def test_gemm_without_vec(lib, ws, epi):
     p.close()
 
 
+@pytest.mark.parametrize("M,N,K", [(2113, 3905, 200), (2100, 4000, 1056), (2304, 3840, 512)])
+@pytest.mark.parametrize("afmt", [FP8, FP4])
+@pytest.mark.parametrize("epi", [EPI_F32, EPI_BF16, EPI_GATED_ADD])
+def test_gemm_large_tiles(lib, ws, M, N, K, afmt, epi):
+    """More than half a round of 256 x 256 tiles, with part tiles and without."""
+    p = Product(M, N, K, afmt, epi, pad=0 if M == 2304 else 1)
+    p.check(p.run(lib, ws.ptr))
+    p.close()
+
+
+@pytest.mark.parametrize("M,N,K", [(2113, 4032, 200), (2304, 4096, 640)])
+@pytest.mark.parametrize("afmt", [FP8, FP4])
+@pytest.mark.parametrize("mx_fmt", [None, FP8, FP4])
+def test_gemm_large_tiles_swiglu(lib, ws, M, N, K, afmt, mx_fmt):
+    p = Product(M, N, K, afmt, EPI_SWIGLU, mx_fmt=mx_fmt)
+    p.check(p.run(lib, ws.ptr))
+    p.close()
+
+
 @pytest.mark.parametrize("M,N,K", [(3, 70, 200), (300, 600, 640), (37, 512, 4096)])
 @pytest.mark.parametrize("afmt", [FP8, FP4])
 def test_gemm_nan_blocks(lib, ws, M, N, K, afmt):
