@@ -175,23 +175,29 @@ struct NormParams {
     uint8_t *q, *s;
     int ldx, ldd, ldxo, ld_q, ld_s, cols, cols_pad;
     float eps;
-    bool vx, vd, vo;   /* 16-byte accesses to x, d, x_out */
+    bool vx, vd, vo, vg, vw, vs;   /* 16-byte accesses to x, d, x_out, gate, w, scale */
 };
 
 __device__ __forceinline__ float to_odd(double y) {
     const float h = (float)y;
     uint32_t u = __float_as_uint(h);
     if (fabs((double)h) > fabs(y)) u--;         /* toward zero; an infinity becomes the largest number */
-    if ((double)h != y) u |= 1;
-    return isnan(y) ? h : __uint_as_float(u);
+    if ((double)h != y) u |= 1;                 /* a NaN stays one */
+    return __uint_as_float(u);
 }
 
 template <int DT> __device__ __forceinline__ Row8 norm_row8(const NormParams &P, size_t row, int c, bool store) {
     Row8 x = load8<false>(P.x + row * P.ldx, c, P.cols, P.vx);
     if constexpr (DT) {
         const Row8 d = load8<DT == 2>((const char *)P.d + row * P.ldd * (DT == 2 ? 2 : 4), c, P.cols, P.vd);
+        if (P.gate) {
+            const Row8 g = load8<false>(P.gate, c, P.cols, P.vg);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x.v[i] = P.gate ? fmaf(c + i < P.cols ? P.gate[c + i] : 0.0f, d.v[i], x.v[i]) : x.v[i] + d.v[i];
+            for (int i = 0; i < 8; i++) x.v[i] = fmaf(g.v[i], d.v[i], x.v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x.v[i] += d.v[i];
+        }
         if (store) {
             float *o = P.x_out + row * P.ldxo + c;
             if (P.vo && c + 8 <= P.cols) {
@@ -239,14 +245,18 @@ template <int FMT, int DT, int R> __global__ __launch_bounds__(NT) void mx_rmsno
     for (int i = 0; i < NT / IRIS_WAVE; i++) ss += red[i];
     const double inv = 1.0 / sqrt(ss / P.cols + (double)P.eps);
     auto put = [&](const Row8 &x, int c) {
+        const Row8 w = load8<false>(P.w, c, P.cols, P.vw);   /* zeros past the row's end */
+        double v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (double)x.v[i] * inv * (double)w.v[i];
+        if (P.scale) {
+            const Row8 g = load8<false>(P.scale, c, P.cols, P.vs);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] *= (double)g.v[i];
+        }
         Row8 y;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const bool in = c + i < P.cols;
-            double v = (double)x.v[i] * inv * (double)(in ? P.w[c + i] : 0.0f);
-            if (P.scale) v *= (double)(in ? P.scale[c + i] : 0.0f);
-            y.v[i] = in ? to_odd(v) : 0.0f;
-        }
+        for (int i = 0; i < 8; i++) y.v[i] = c + i < P.cols ? to_odd(v[i]) : 0.0f;   /* 0 inv may be NaN */
         mx_put8<FMT>(P.q + row * P.ld_q, P.s + row * P.ld_s, c, y);
     };
     if constexpr (R > 0) {
@@ -1100,6 +1110,9 @@ extern "C" int iris_hip_mx_rmsnorm(const iris_mx_norm_t *a) {
     P.vx = rows16(a->x, a->ldx, 4);
     P.vd = rows16(a->d, a->ldd, a->d_bf16 ? 2 : 4);
     P.vo = rows16(a->x_out, a->ldxo, 4);
+    P.vg = rows16(a->gate, 0, 4);
+    P.vw = rows16(a->w, 0, 4);
+    P.vs = rows16(a->scale, 0, 4);
     const int dt = !a->d ? 0 : a->d_bf16 ? 2 : 1;
     if (a->out.fmt == IRIS_MX_FP8) {
         if (dt == 0) launch_norm<IRIS_MX_FP8, 0>(P, a->rows);
