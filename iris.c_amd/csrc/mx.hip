@@ -435,20 +435,216 @@ __device__ __forceinline__ void mx_store_swiglu(const MxGemm &P, int m, int n, c
         }
 }
 
+constexpr int waitcnt_imm(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
+typedef __attribute__((address_space(3))) void lds_void;
+constexpr int GROUP_M = 8;
+
+
+/* 64 lanes' 16 bytes from a buffer to LDS, one after the other from place at on
+ * (rows past the buffer's end: zeros). Not the builtin: before reads of one
+ * stage the compiler waits for the builtin's loads into the others too, which
+ * takes the ring's depth away. The caller waits (vmcnt) before a barrier. */
+__device__ __forceinline__ uint32_t lds_at(const void *p) { return (uint32_t)(uintptr_t)(const lds_void *)p; }
+__device__ __forceinline__ void load_lds16(const u32x4 &rsrc, uint32_t at, int voff, int soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 ::"s"(at), "v"(voff), "s"(rsrc), "s"(soff)
+                 : "memory");
+}
+__device__ __forceinline__ u32x4 buffer_of(const void *p, int bytes) {
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    return (u32x4){(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)),
+                   (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+}
+
+/* byte j of word i to byte i of word j */
+__device__ __forceinline__ u32x4 bytes4x4(const u32x4 &x) {
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400), b = __builtin_amdgcn_perm(x[1], x[0], 0x07030602);
+    const uint32_t c = __builtin_amdgcn_perm(x[3], x[2], 0x05010400), d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602);
+    return (u32x4){__builtin_amdgcn_perm(c, a, 0x05040100), __builtin_amdgcn_perm(c, a, 0x07060302),
+                   __builtin_amdgcn_perm(d, b, 0x05040100), __builtin_amdgcn_perm(d, b, 0x07060302)};
+}
+
+template <int V> struct Const {
+    static constexpr int value = V;
+};
+
+#define WAIT(vm, lgkm)                                              \
+    do {                                                            \
+        __builtin_amdgcn_sched_barrier(0);                          \
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(vm, lgkm));          \
+        __builtin_amdgcn_sched_barrier(0);                          \
+    } while (0)
+
 /* ---- product of few rows ----
- * Bound by W's bytes, not by the matrix instructions. A block's 8 waves share
- * 16 FM rows of A and 16 FN of W and take consecutive parts of K, fragments
- * straight from global memory, U steps of 128 in flight per wave: 16 rows of W
- * and one of A keep 8 waves x 4 KiB in flight. The waves' sums are added in
- * wave order through LDS. */
-template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm_rows_kernel(MxGemm P) {
-    constexpr int U = FM * FN == 1 ? 4 : FM == 1 ? 3 : 2;
-    extern __shared__ f32x4 part[];   /* [8 waves][FM * FN tiles][64 lanes] */
+ * Bound by W's bytes and by the number of 128-byte lines that loads touch (1.5
+ * ns each and CU), not by the matrix instructions. A block's waves share 16 FM
+ * rows of A and 16 FN of W; a wave takes every waves-th unit of 256 columns,
+ * through a part of LDS of its own: loads of 8 rows x 128 bytes, straight into
+ * LDS (16-byte chunks XORed with the row number, as in the tiles below), while
+ * the unit before is multiplied. Fragments straight from global memory touch
+ * each line twice, and a wave's loads in registers leave room for half the
+ * waves: gate and up of 37 rows 24.8 us. Scales of 4096 columns are loaded by
+ * the whole block, a line a row. The waves' sums are added in wave order. */
+template <int AF, int FM, int FN> struct RowsShape {
+    static constexpr int A_ROW = AF == IRIS_MX_FP8 ? 256 : 128;    /* bytes of 256 columns */
+    static constexpr int A_BYTES = FM * 16 * A_ROW, UNIT = A_BYTES + FN * 2048;
+    static constexpr int SCALES = 16 * (FM + FN) * 128;            /* bytes of 4096 columns */
+    static constexpr int fit(int bytes) { return bytes / UNIT > 16 ? 16 : bytes / UNIT; }
+    static constexpr int WAVES = fit(163840 - SCALES), WAVES2 = fit(81920 - SCALES);   /* one block per CU, two */
+};
+
+template <int AF, int FM, int FN>
+__global__ __launch_bounds__((64 * RowsShape<AF, FM, FN>::WAVES)) void mx_gemm_rows_kernel(MxGemm P) {
+    using Sh = RowsShape<AF, FM, FN>;
+    constexpr bool F8 = AF == IRIS_MX_FP8;
+    constexpr int SEG = 32;                    /* steps whose scales are in LDS */
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   /* scales, then a unit per wave; sums at the end */
+    const int tiles = P.tiles_m * P.tiles_n;
+    const int chunk = (int)blockIdx.x / tiles, t = (int)blockIdx.x - chunk * tiles;
+    const int off = chunk * P.per_chunk;
+    mx_chunk<AF>(P, chunk);
+    const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
+    const int m0 = t / P.tiles_n * 16 * FM, n0 = t % P.tiles_n * 16 * FN;
+    const int a_rows = min(16 * FM, P.M - m0), w_rows = min(16 * FN, P.N - n0);
+    /* rows past the end read as zeros */
+    const u32x4 a_rsrc = buffer_of(P.aq + (size_t)m0 * P.lda, a_rows * P.lda - off * (F8 ? 128 : 64));
+    const u32x4 w_rsrc = buffer_of(P.wq + (size_t)n0 * P.ldw, w_rows * P.ldw - off * 64);
+    const u32x4 as_rsrc = buffer_of(P.as + (size_t)m0 * P.ldas, a_rows * P.ldas - off * 4);
+    const u32x4 ws_rsrc = buffer_of(P.ws + (size_t)n0 * P.ldws, w_rows * P.ldws - off * 4);
+    uint8_t *const mine = lds + Sh::SCALES + wave * Sh::UNIT;
+    const uint32_t scl0 = lds_at(lds), at0 = lds_at(mine);
+    const int units = (P.steps + 1) / 2;
+
+    /* a load of 8 rows x 128 bytes: lane l row l / 8, place l % 8, chunk place
+     * ^ (row % 8); chunks: how many of the 8 lie within the row's data, the
+     * others read the first */
+    const int row8 = lane >> 3, ch8 = (lane & 7) ^ row8;
+    auto load8rows = [&](const u32x4 &rsrc, uint32_t at, int row0, int ld, int soff, int chunks) {
+        load_lds16(rsrc, at, (row0 + row8) * ld + (ch8 < chunks ? ch8 << 4 : 0), soff);
+    };
+    auto load_unit = [&](int u) {
+        const int n = min(2, P.steps - 2 * u);   /* steps of 128 columns */
+#pragma unroll
+        for (int i = 0; i < 2 * FN; i++)
+            if (8 * i < w_rows) load8rows(w_rsrc, at0 + Sh::A_BYTES + i * 1024, 8 * i, P.ldw, u * 128, 4 * n);
+#pragma unroll
+        for (int i = 0; i < 2 * FM; i++)
+            if (8 * i < a_rows) {
+                load8rows(a_rsrc, at0 + i * 1024, 8 * i, P.lda, u * Sh::A_ROW, F8 ? 8 : 4 * n);
+                if (F8 && n == 2) load8rows(a_rsrc, at0 + FM * 2048 + i * 1024, 8 * i, P.lda, u * 256 + 128, 8);
+            }
+    };
+    auto load_scales = [&](int seg) {
+        const int chunks = min(8, (P.steps - seg * SEG + 3) / 4);
+        for (int i = wave; i < 2 * (FM + FN); i += waves) {
+            if (i < 2 * FM) {
+                if (8 * i < a_rows) load8rows(as_rsrc, scl0 + i * 1024, 8 * i, P.ldas, seg * 128, chunks);
+            } else if (8 * i - 16 * FM < w_rows) load8rows(ws_rsrc, scl0 + i * 1024, 8 * i - 16 * FM, P.ldws, seg * 128, chunks);
+        }
+    };
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    /* places of a fragment row's chunk c, and of its scale byte of step k: rows 16 apart are stored alike */
+    const int frow = lr * 128;
+    auto piece = [&](int c) { return frow + ((c ^ (lr & 7)) << 4); };
+    auto scale = [&](int tile, int k) { return (int)lds[tile * 2048 + piece((k & (SEG - 1)) >> 2) + (k & 3) * 4 + lg]; };
+    auto unit = [&](int u, int n, int next) {
+        u32x4 w[2][FN], a[2][FM][2];
+        int sw[2][FN], sa[2][FM];
+        WAIT(0, 15);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if (h >= n) break;
+#pragma unroll
+            for (int j = 0; j < FN; j++) {
+                w[h][j] = *(const u32x4 *)(mine + Sh::A_BYTES + j * 2048 + piece(4 * h + lg));
+                sw[h][j] = scale(FM + j, 2 * u + h);
+            }
+#pragma unroll
+            for (int i = 0; i < FM; i++) {
+                const uint8_t *x = mine + (F8 ? h * FM * 2048 : 0) + i * 2048;
+                a[h][i][0] = *(const u32x4 *)(x + piece(F8 ? lg : 4 * h + lg));
+                a[h][i][1] = F8 ? *(const u32x4 *)(x + piece(4 + lg)) : (u32x4){0, 0, 0, 0};
+                sa[h][i] = scale(i, 2 * u + h);
+            }
+        }
+        WAIT(63, 0);
+        if (next >= 0) load_unit(next);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if (h >= n) break;
+#pragma unroll
+            for (int i = 0; i < FM; i++) {
+                const u32x4 x = a[h][i][0], y = a[h][i][1];
+                const i32x8 x8 = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+                const i32x8 hi = F8 ? mx_part<true>(x8) : x8, lo = mx_part<false>(x8);
+#pragma unroll
+                for (int j = 0; j < FN; j++) {
+                    acc[i][j] = mx_mfma<AF>(w[h][j], hi, acc[i][j], sw[h][j], sa[h][i]);
+                    if constexpr (F8) acc[i][j] = mx_mfma<AF>(w[h][j], lo, acc[i][j], sw[h][j], sa[h][i]);
+                }
+            }
+        }
+    };
+    int u = wave;
+    if (u < units) load_unit(u);
+    for (int seg = 0; seg * SEG < P.steps; seg++) {
+        if (seg) __syncthreads();   /* everyone is done with the scales before */
+        load_scales(seg);
+        WAIT(0, 0);
+        __syncthreads();
+        const int end = min(units, (seg + 1) * (SEG / 2));
+        for (; u < end; u += waves) {
+            const int next = u + waves < units ? u + waves : -1;
+            if (2 * u + 1 < P.steps) unit(u, 2, next);
+            else unit(u, 1, next);
+        }
+    }
+    __syncthreads();
+    f32x4 *const part = (f32x4 *)lds;   /* [waves][FM * FN tiles][64 lanes] */
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) part[(wave * FM * FN + i * FN + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    auto sum = [&](int i, int j) {
+        f32x4 s = part[(i * FN + j) * 64 + lane];
+        for (int w = 1; w < waves; w++) s += part[(w * FM * FN + i * FN + j) * 64 + lane];
+        return s;
+    };
+    const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
+    if constexpr (FN == 4) {
+        if (P.epi == IRIS_EPI_SWIGLU) {
+            for (int i = wave; i < FM; i += waves)
+                mx_store_swiglu(P, m0 + 16 * i + lr, n0, sum(i, 0), sum(i, 1), sum(i, 2), sum(i, 3), aligned);
+            return;
+        }
+    }
+    for (int q = wave; q < FM * FN; q += waves) {
+        const int m = m0 + 16 * (q / FN) + lr;
+        const f32x4 s = sum(q / FN, q % FN);
+        if (m < P.M) mx_store4(P, m, n0 + 16 * (q % FN) + 4 * lg, s, aligned);
+    }
+}
+
+/* ---- product without LDS staging ----
+ * Fragments straight from global memory by 64-bit pointers, a wave per group
+ * of 512 columns in turn: for one to 16 rows of A (plain epilogues), and for
+ * rows further apart than the other kernels' 32-bit offsets reach. Whole
+ * 128-byte lines of the codes and one 16-byte load of scales a row for 4
+ * steps (a 4-byte load per step touched as many lines as W). */
+template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm_direct_kernel(MxGemm P) {
+    extern __shared__ f32x4 part[];   /* [waves][FM * FN tiles][64 lanes] */
     const int tiles = P.tiles_m * P.tiles_n;
     const int chunk = (int)blockIdx.x / tiles, t = (int)blockIdx.x - chunk * tiles;
     mx_chunk<AF>(P, chunk);
     const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
     const int m0 = t / P.tiles_n * 16 * FM, n0 = t % P.tiles_n * 16 * FN;
     const uint8_t *ap[FM], *sap[FM], *wp[FN], *swp[FN];
 #pragma unroll
@@ -468,44 +664,48 @@ template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm
     for (int i = 0; i < FM; i++)
 #pragma unroll
         for (int j = 0; j < FN; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    const int per = (P.steps + 7) / 8, k1 = min((wave + 1) * per, P.steps);
-    for (int k0 = wave * per; k0 < k1; k0 += U) {
-        u32x4 w[U][FN], a[U][FM][2];
-        uint32_t sw[U][FN], sa[U][FM];
+    /* steps 4 g .. 4 g + n - 1 */
+    auto group = [&](int g, int n) {
+        u32x4 sw[FN], sa[FM], w[4][FN], a[4][FM][2];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int k = min(k0 + u, k1 - 1);
+        for (int j = 0; j < FN; j++) sw[j] = *(const u32x4 *)(swp[j] + (size_t)g * 16);
 #pragma unroll
-            for (int j = 0; j < FN; j++) {
-                w[u][j] = *(const u32x4 *)(wp[j] + (size_t)k * 64);
-                sw[u][j] = *(const uint32_t *)(swp[j] + k * 4);
-            }
+        for (int i = 0; i < FM; i++) sa[i] = *(const u32x4 *)(sap[i] + (size_t)g * 16);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (u >= n) break;
+            const size_t k = (size_t)g * 4 + u;
+#pragma unroll
+            for (int j = 0; j < FN; j++) w[u][j] = *(const u32x4 *)(wp[j] + k * 64);
 #pragma unroll
             for (int i = 0; i < FM; i++) {
-                const uint8_t *x = ap[i] + (size_t)k * (AF == IRIS_MX_FP8 ? 128 : 64);
+                const uint8_t *x = ap[i] + k * (AF == IRIS_MX_FP8 ? 128 : 64);
                 a[u][i][0] = *(const u32x4 *)x;
                 a[u][i][1] = AF == IRIS_MX_FP8 ? *(const u32x4 *)(x + 64) : (u32x4){0, 0, 0, 0};
-                sa[u][i] = *(const uint32_t *)(sap[i] + k * 4);
             }
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (k0 + u >= k1) break;
+        for (int u = 0; u < 4; u++) {
+            if (u >= n) break;
 #pragma unroll
             for (int i = 0; i < FM; i++) {
                 const u32x4 x = a[u][i][0], y = a[u][i][1];
                 const i32x8 x8 = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
                 const i32x8 hi = AF == IRIS_MX_FP8 ? mx_part<true>(x8) : x8, lo = mx_part<false>(x8);
-                const int s = (int)(sa[u][i] >> 8 * lg);
+                const int s = (int)(sa[i][u] >> 8 * lg);
 #pragma unroll
                 for (int j = 0; j < FN; j++) {
-                    const int r = (int)(sw[u][j] >> 8 * lg);
+                    const int r = (int)(sw[j][u] >> 8 * lg);
                     acc[i][j] = mx_mfma<AF>(w[u][j], hi, acc[i][j], r, s);
                     if constexpr (AF == IRIS_MX_FP8) acc[i][j] = mx_mfma<AF>(w[u][j], lo, acc[i][j], r, s);
                 }
             }
         }
-    }
+    };
+    const int whole = P.steps / 4;
+    int g = wave;
+    for (; g < whole; g += waves) group(g, 4);
+    if (g == whole && (P.steps & 3)) group(g, P.steps & 3);
 #pragma unroll
     for (int i = 0; i < FM; i++)
 #pragma unroll
@@ -513,18 +713,18 @@ template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm
     __syncthreads();
     auto sum = [&](int i, int j) {
         f32x4 s = part[(i * FN + j) * 64 + lane];
-#pragma unroll
-        for (int w = 1; w < 8; w++) s += part[(w * FM * FN + i * FN + j) * 64 + lane];
+        for (int w = 1; w < waves; w++) s += part[(w * FM * FN + i * FN + j) * 64 + lane];
         return s;
     };
     const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
     if constexpr (FN == 4) {
         if (P.epi == IRIS_EPI_SWIGLU) {
-            if (wave < FM) mx_store_swiglu(P, m0 + 16 * wave + lr, n0, sum(wave, 0), sum(wave, 1), sum(wave, 2), sum(wave, 3), aligned);
+            for (int i = wave; i < FM; i += waves)
+                mx_store_swiglu(P, m0 + 16 * i + lr, n0, sum(i, 0), sum(i, 1), sum(i, 2), sum(i, 3), aligned);
             return;
         }
     }
-    for (int q = wave; q < FM * FN; q += 8) {
+    for (int q = wave; q < FM * FN; q += waves) {
         const int m = m0 + 16 * (q / FN) + lr;
         const f32x4 s = sum(q / FN, q % FN);
         if (m < P.M) mx_store4(P, m, n0 + 16 * (q % FN) + 4 * lg, s, aligned);
@@ -599,40 +799,7 @@ __global__ __launch_bounds__(NT) void mx_reduce_kernel(const MxGemm P, const flo
  * are, then a lane transposes the 4 x 4 bytes of a row so that the bytes of
  * lane group g (block g of each 128 columns) make one word; a fragment's lane
  * reads its word once per 512 columns and shifts it by a byte per 128. */
-constexpr int waitcnt_imm(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
-typedef __attribute__((address_space(3))) void lds_void;
-constexpr int GROUP_M = 8;
-
-
-/* 64 lanes' 16 bytes from a buffer to LDS, one after the other from place at on
- * (rows past the buffer's end: zeros). Not the builtin: before reads of one
- * stage the compiler waits for the builtin's loads into the others too, which
- * takes the ring's depth away. The caller waits (vmcnt) before a barrier. */
-__device__ __forceinline__ uint32_t lds_at(const void *p) { return (uint32_t)(uintptr_t)(const lds_void *)p; }
-__device__ __forceinline__ void load_lds16(const u32x4 &rsrc, uint32_t at, int voff, int soff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 ::"s"(at), "v"(voff), "s"(rsrc), "s"(soff)
-                 : "memory");
-}
-__device__ __forceinline__ u32x4 buffer_of(const void *p, int bytes) {
-    const uint64_t a = (uint64_t)(uintptr_t)p;
-    return (u32x4){(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)),
-                   (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
-}
-
-/* byte j of word i to byte i of word j */
-__device__ __forceinline__ u32x4 bytes4x4(const u32x4 &x) {
-    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400), b = __builtin_amdgcn_perm(x[1], x[0], 0x07030602);
-    const uint32_t c = __builtin_amdgcn_perm(x[3], x[2], 0x05010400), d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602);
-    return (u32x4){__builtin_amdgcn_perm(c, a, 0x05040100), __builtin_amdgcn_perm(c, a, 0x07060302),
-                   __builtin_amdgcn_perm(d, b, 0x05040100), __builtin_amdgcn_perm(d, b, 0x07060302)};
-}
-
 __device__ __forceinline__ bool rows16_ok(const void *p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0; }
-
-template <int V> struct Const {
-    static constexpr int value = V;
-};
 
 template <int AF, bool SPLIT, int BM, int BN>
 __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(MxGemm P) {
@@ -789,12 +956,6 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
 #pragma unroll
             for (int j = 0; j < FN; j++) asm volatile("" ::"v"(acc[i][j]));
     };
-#define WAIT(vm, lgkm)                                              \
-    do {                                                            \
-        __builtin_amdgcn_sched_barrier(0);                          \
-        __builtin_amdgcn_s_waitcnt(waitcnt_imm(vm, lgkm));          \
-        __builtin_amdgcn_sched_barrier(0);                          \
-    } while (0)
     auto barrier = [&]() {
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_barrier();
@@ -903,7 +1064,6 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
         }
     }
     WAIT(0, 0);   /* no load outstanding at exit */
-#undef WAIT
     const int lane = hidden_lane(), lr = lane & 15, lg = lane >> 4;
     /* Whole tiles of 16-bit or microscaled output leave through LDS, two of a
      * wave's 16-row tiles at a time, so that a row's part of a wave (256, 128
@@ -1128,26 +1288,40 @@ extern "C" int iris_hip_mx_rmsnorm(const iris_mx_norm_t *a) {
 
 /* ---- which kernel, and whether K is split ---- */
 namespace {
-enum { MX_ROWS, MX_TILE128, MX_TILE256 };
+enum { MX_ROWS, MX_DIRECT, MX_TILE128, MX_TILE256 };
 struct MxPlan {
     int kind, fm, fn, tiles_m, tiles_n, chunks, per_chunk;
 };
 
 template <int AF, int FM, int FN> int launch_rows_of(const MxGemm &P, unsigned blocks) {
-    constexpr int smem = 8 * FM * FN * 1024;
+    using Sh = RowsShape<AF, FM, FN>;
+    /* units of 256 columns, as evenly as the waves that LDS holds take them */
+    const int most = (int)blocks <= iris_cu_count() ? Sh::WAVES : Sh::WAVES2;
+    const int units = (P.per_chunk + 1) / 2, rounds = (units + most - 1) / most;
+    const int waves = (units + rounds - 1) / rounds;
+    const int smem = Sh::SCALES + waves * Sh::UNIT;
+    static_assert(Sh::UNIT >= FM * FN * 1024, "the sums fit where the units were");
     static std::once_flag once;
     static hipError_t attr = hipSuccess;
     std::call_once(once, [] {
-        attr = hipFuncSetAttribute((const void *)mx_gemm_rows_kernel<AF, FM, FN>, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+        attr = hipFuncSetAttribute((const void *)mx_gemm_rows_kernel<AF, FM, FN>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   Sh::SCALES + Sh::WAVES * Sh::UNIT);
     });
     if (iris_check(attr, "mx_gemm_rows smem attribute")) return -1;
-    IRIS_LAUNCH((mx_gemm_rows_kernel<AF, FM, FN>), dim3(blocks), dim3(512), smem, iris_stream(), P);
+    IRIS_LAUNCH((mx_gemm_rows_kernel<AF, FM, FN>), dim3(blocks), dim3(64 * waves), smem, iris_stream(), P);
     return 0;
 }
 template <int AF> int launch_rows(const MxGemm &P, const MxPlan &plan, unsigned blocks) {
-    if (plan.fn == 1) return launch_rows_of<AF, 1, 1>(P, blocks);
+    if (plan.kind == MX_DIRECT) {
+        /* a wave per 512 columns, as evenly as 8 waves take them */
+        const int groups = (P.per_chunk + 3) / 4, rounds = (groups + 7) / 8, waves = (groups + rounds - 1) / rounds;
+        if (plan.fn == 1) IRIS_LAUNCH((mx_gemm_direct_kernel<AF, 1, 1>), dim3(blocks), dim3(64 * waves), waves * 1024, iris_stream(), P);
+        else IRIS_LAUNCH((mx_gemm_direct_kernel<AF, 1, 4>), dim3(blocks), dim3(64 * waves), waves * 4096, iris_stream(), P);
+        return 0;
+    }
     if (plan.fm == 1) return launch_rows_of<AF, 1, 4>(P, blocks);
     if (plan.fm == 2) return launch_rows_of<AF, 2, 4>(P, blocks);
+    if (plan.fm == 3) return launch_rows_of<AF, 3, 4>(P, blocks);
     return launch_rows_of<AF, 4, 4>(P, blocks);
 }
 
@@ -1160,9 +1334,12 @@ MxPlan mx_plan(const iris_mx_gemm_t &p, int steps, size_t ws_bytes) {
     const bool far = ld * 256 > 0x7fffffffLL;
     int bm, bn;
     if (p.M <= 64 || far) {
-        q.kind = MX_ROWS;
-        q.fm = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-        q.fn = q.fm == 1 && p.epi != IRIS_EPI_SWIGLU ? 1 : 4;
+        /* 16 rows of A at most: 16 of W per block keep enough blocks in flight
+         * without LDS (6144 x 2560, one row: 4.9 us, 5.4 through LDS); a gate
+         * / up group needs 64 */
+        q.fn = p.epi == IRIS_EPI_SWIGLU || p.M > 16 ? 4 : 1;
+        q.kind = far || q.fn == 1 ? MX_DIRECT : MX_ROWS;
+        q.fm = q.kind == MX_DIRECT ? 1 : (p.M + 15) / 16;
         bm = 16 * q.fm;
         bn = 16 * q.fn;
     } else {
@@ -1221,7 +1398,7 @@ extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_by
         P.out = ws; P.ldo = p->N; P.vec = nullptr; P.epi = IRIS_EPI_F32; P.oq = nullptr;
     }
     const bool f8 = p->A.fmt == IRIS_MX_FP8;
-    if (plan.kind == MX_ROWS) {
+    if (plan.kind <= MX_DIRECT) {
         if (f8 ? launch_rows<IRIS_MX_FP8>(P, plan, (unsigned)blocks) : launch_rows<IRIS_MX_FP4>(P, plan, (unsigned)blocks)) return -1;
     } else {
         /* 16- and 8-bit results are rounded 100 times coarser than what the
