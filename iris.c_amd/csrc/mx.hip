@@ -71,18 +71,20 @@ template <int FMT> __device__ __forceinline__ void mx_put8(uint8_t *q, uint8_t *
 }
 
 /* 8 columns from c on of a row of f32 or bf16, zeros past cols; vec: 16-byte accesses are allowed */
-template <bool BF16> __device__ __forceinline__ Row8 load8(const void *row, int c, int cols, bool vec) {
+template <bool BF16, bool STREAM = false> __device__ __forceinline__ Row8 load8(const void *row, int c, int cols, bool vec) {
     Row8 x;
     if (vec && c + 8 <= cols) {
         if constexpr (BF16) {
-            const u32x4 t = *(const u32x4 *)((const uint16_t *)row + c);
+            const u32x4 *p = (const u32x4 *)((const uint16_t *)row + c);
+            const u32x4 t = STREAM ? __builtin_nontemporal_load(p) : *p;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 x.v[2 * i] = __uint_as_float(t[i] << 16);
                 x.v[2 * i + 1] = __uint_as_float(t[i] & 0xffff0000u);
             }
         } else {
-            const float4 a = *(const float4 *)((const float *)row + c), b = *(const float4 *)((const float *)row + c + 4);
+            const float4 *p = (const float4 *)((const float *)row + c);
+            const float4 a = STREAM ? ld_stream(p) : p[0], b = STREAM ? ld_stream(p + 1) : p[1];
             x.v[0] = a.x; x.v[1] = a.y; x.v[2] = a.z; x.v[3] = a.w;
             x.v[4] = b.x; x.v[5] = b.y; x.v[6] = b.z; x.v[7] = b.w;
         }
@@ -187,9 +189,9 @@ __device__ __forceinline__ float to_odd(double y) {
 }
 
 template <int DT> __device__ __forceinline__ Row8 norm_row8(const NormParams &P, size_t row, int c, bool store) {
-    Row8 x = load8<false>(P.x + row * P.ldx, c, P.cols, P.vx);
+    Row8 x = load8<false, DT != 0>(P.x + row * P.ldx, c, P.cols, P.vx);
     if constexpr (DT) {
-        const Row8 d = load8<DT == 2>((const char *)P.d + row * P.ldd * (DT == 2 ? 2 : 4), c, P.cols, P.vd);
+        const Row8 d = load8<DT == 2, true>((const char *)P.d + row * P.ldd * (DT == 2 ? 2 : 4), c, P.cols, P.vd);
         if (P.gate) {
             const Row8 g = load8<false>(P.gate, c, P.cols, P.vg);
 #pragma unroll
