@@ -13,6 +13,7 @@
  */
 #include "iris_internal.h"
 
+#include <math.h>
 #include <mutex>
 
 namespace {
@@ -71,20 +72,18 @@ template <int FMT> __device__ __forceinline__ void mx_put8(uint8_t *q, uint8_t *
 }
 
 /* 8 columns from c on of a row of f32 or bf16, zeros past cols; vec: 16-byte accesses are allowed */
-template <bool BF16, bool STREAM = false> __device__ __forceinline__ Row8 load8(const void *row, int c, int cols, bool vec) {
+template <bool BF16> __device__ __forceinline__ Row8 load8(const void *row, int c, int cols, bool vec) {
     Row8 x;
     if (vec && c + 8 <= cols) {
         if constexpr (BF16) {
-            const u32x4 *p = (const u32x4 *)((const uint16_t *)row + c);
-            const u32x4 t = STREAM ? __builtin_nontemporal_load(p) : *p;
+            const u32x4 t = *(const u32x4 *)((const uint16_t *)row + c);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 x.v[2 * i] = __uint_as_float(t[i] << 16);
                 x.v[2 * i + 1] = __uint_as_float(t[i] & 0xffff0000u);
             }
         } else {
-            const float4 *p = (const float4 *)((const float *)row + c);
-            const float4 a = STREAM ? ld_stream(p) : p[0], b = STREAM ? ld_stream(p + 1) : p[1];
+            const float4 a = *(const float4 *)((const float *)row + c), b = *(const float4 *)((const float *)row + c + 4);
             x.v[0] = a.x; x.v[1] = a.y; x.v[2] = a.z; x.v[3] = a.w;
             x.v[4] = b.x; x.v[5] = b.y; x.v[6] = b.z; x.v[7] = b.w;
         }
@@ -189,9 +188,9 @@ __device__ __forceinline__ float to_odd(double y) {
 }
 
 template <int DT> __device__ __forceinline__ Row8 norm_row8(const NormParams &P, size_t row, int c, bool store) {
-    Row8 x = load8<false, DT != 0>(P.x + row * P.ldx, c, P.cols, P.vx);
+    Row8 x = load8<false>(P.x + row * P.ldx, c, P.cols, P.vx);
     if constexpr (DT) {
-        const Row8 d = load8<DT == 2, true>((const char *)P.d + row * P.ldd * (DT == 2 ? 2 : 4), c, P.cols, P.vd);
+        const Row8 d = load8<DT == 2>((const char *)P.d + row * P.ldd * (DT == 2 ? 2 : 4), c, P.cols, P.vd);
         if (P.gate) {
             const Row8 g = load8<false>(P.gate, c, P.cols, P.vg);
 #pragma unroll
@@ -203,8 +202,9 @@ template <int DT> __device__ __forceinline__ Row8 norm_row8(const NormParams &P,
         if (store) {
             float *o = P.x_out + row * P.ldxo + c;
             if (P.vo && c + 8 <= P.cols) {
-                *(float4 *)o = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
-                *(float4 *)(o + 4) = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
+                /* streaming: 4608 x 3840 that no cache holds 51 -> 46 us */
+                st_stream((float4 *)o, make_float4(x.v[0], x.v[1], x.v[2], x.v[3]));
+                st_stream((float4 *)(o + 4), make_float4(x.v[4], x.v[5], x.v[6], x.v[7]));
             } else
 #pragma unroll
                 for (int i = 0; i < 8; i++)
@@ -1327,44 +1327,89 @@ template <int AF> int launch_rows(const MxGemm &P, const MxPlan &plan, unsigned 
     return launch_rows_of<AF, 4, 4>(P, blocks);
 }
 
+/* The kernel, the tile and the number of K ranges of least estimated time (us),
+ * fitted to 130 products of 20 to 1500 rows (within 1.5 % of the fastest
+ * measured choice on average, 25 % at most). A launch with its first loads and
+ * last stores is 6; a round of 256 x 256 tiles 3 and per K step 0.85 (e2m1 A),
+ * 1.25 (e4m3) or 2.85 (e4m3, f32 sums); one of 128 x 128 tiles 2 and 0.32,
+ * 0.41 or 0.72: for f32 sums never slower, as the instructions bound both. A
+ * split's partial sums and their second launch are 3 and their bytes at 4 TB/s.
+ * Measured, us: 300 x 19456 x 2560 e4m3 to bf16: 24.1 on 128 x 128 tiles, 31.6
+ * on 256 x 256; 512 rows 32.7 and 28.7; 512 x 2560 x 9728 to f32: 63 unsplit,
+ * 36.6 in 3 ranges; 64 x 6144 x 2560: 12.8 through mx_gemm_rows_kernel, 14.4
+ * on tiles; 64 x 19456 x 2560: 22.2 and 16.2. */
+template <int AF> void rows_waves(int fm, int *one, int *two) {
+    switch (fm) {
+    case 1: *one = RowsShape<AF, 1, 4>::WAVES; *two = RowsShape<AF, 1, 4>::WAVES2; break;
+    case 2: *one = RowsShape<AF, 2, 4>::WAVES; *two = RowsShape<AF, 2, 4>::WAVES2; break;
+    case 3: *one = RowsShape<AF, 3, 4>::WAVES; *two = RowsShape<AF, 3, 4>::WAVES2; break;
+    default: *one = RowsShape<AF, 4, 4>::WAVES; *two = RowsShape<AF, 4, 4>::WAVES2; break;
+    }
+}
+
+bool mx_exact(const iris_mx_gemm_t &p) {
+    /* 16- and 8-bit results are rounded 100 times coarser than what the single
+     * instruction loses; f32 results get f32 sums */
+    return p.A.fmt == IRIS_MX_FP8 && p.epi != IRIS_EPI_SWIGLU && p.epi != IRIS_EPI_BF16;
+}
+
 MxPlan mx_plan(const iris_mx_gemm_t &p, int steps, size_t ws_bytes) {
-    const int cus = iris_cu_count();
-    MxPlan q;
-    /* tile loads reach rows by 32-bit offsets */
+    const int cus = iris_cu_count() > 0 ? iris_cu_count() : 1;
+    /* the staging kernels reach rows by 32-bit offsets */
     long long ld = p.A.ld_q;
     for (int v : {p.W.ld_q, p.A.ld_s, p.W.ld_s}) ld = v > ld ? v : ld;
     const bool far = ld * 256 > 0x7fffffffLL;
-    int bm, bn;
-    if (p.M <= 64 || far) {
-        /* 16 rows of A at most: 16 of W per block keep enough blocks in flight
-         * without LDS (6144 x 2560, one row: 4.9 us, 5.4 through LDS); a gate
-         * / up group needs 64 */
-        q.fn = p.epi == IRIS_EPI_SWIGLU || p.M > 16 ? 4 : 1;
-        q.kind = far || q.fn == 1 ? MX_DIRECT : MX_ROWS;
-        q.fm = q.kind == MX_DIRECT ? 1 : (p.M + 15) / 16;
-        bm = 16 * q.fm;
-        bn = 16 * q.fn;
-    } else {
-        const long long t256 = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
-        q.kind = t256 * 2 > cus ? MX_TILE256 : MX_TILE128;
-        bm = bn = q.kind == MX_TILE256 ? 256 : 128;
-    }
-    q.tiles_m = (p.M + bm - 1) / bm;
-    q.tiles_n = (p.N + bn - 1) / bn;
-    q.chunks = 1;
-    q.per_chunk = steps;
-    const long long tiles = (long long)q.tiles_m * q.tiles_n;
-    if (ws_bytes && tiles * 2 <= cus && steps >= 16 && (size_t)p.M * ((p.N + 127) / 128 * 16) < (1u << 31)) {
-        long long c = cus / tiles;
-        const long long most = (long long)(ws_bytes / ((size_t)p.M * p.N * 4));
-        if (c > most) c = most;
-        if (c > steps / 8) c = steps / 8;
-        if (c > 1) {
-            q.per_chunk = (int)((steps + c - 1) / c + 3) / 4 * 4;
+    const bool f8 = p.A.fmt == IRIS_MX_FP8;
+    MxPlan best;
+    double least = 0.0;
+    best.chunks = 0;
+    auto consider = [&](int kind, int fm, int fn, int bm, int bn) {
+        MxPlan q;
+        q.kind = kind;
+        q.fm = fm;
+        q.fn = fn;
+        q.tiles_m = (p.M + bm - 1) / bm;
+        q.tiles_n = (p.N + bn - 1) / bn;
+        const double tiles = (double)q.tiles_m * q.tiles_n, mn = (double)p.M * p.N;
+        for (int c : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            q.per_chunk = c == 1 ? steps : ((steps + c - 1) / c + 3) / 4 * 4;
             q.chunks = (steps + q.per_chunk - 1) / q.per_chunk;
+            if (c > 1 && (q.chunks == 1 || q.chunks * mn * 4 > (double)ws_bytes || mn > 1e9)) break;
+            const double blocks = tiles * q.chunks;
+            double us;
+            if (kind == MX_TILE128 || kind == MX_TILE256) {
+                const bool big = kind == MX_TILE256;
+                const double step = !f8 ? (big ? 0.85 : 0.32) : mx_exact(p) ? 0.72 : big ? 1.25 : 0.41;
+                us = 6 + ceil(blocks / cus) * ((big ? 3 : 2) + step * q.per_chunk);
+            } else if (kind == MX_ROWS) {
+                int one, two;
+                if (f8) rows_waves<IRIS_MX_FP8>(fm, &one, &two);
+                else rows_waves<IRIS_MX_FP4>(fm, &one, &two);
+                const int units = (q.per_chunk + 1) / 2, waves = blocks > cus ? two : one;
+                us = 8 + ceil(blocks / (2.0 * cus)) * ((units + waves - 1) / waves) * (1.2 + (f8 ? 0.35 : 0.25) * fm) * (blocks > cus ? 0.85 : 1.0);
+            } else us = 6 + ceil(blocks / (4.0 * cus)) * (q.per_chunk + 31) / 32 * 2.0;   /* 8 waves of 4 steps each */
+            if (q.chunks > 1) us += 3 + q.chunks * mn * 8 / 4e6;
+            if (!best.chunks || us < least) {
+                best = q;
+                least = us;
+            }
+        }
+    };
+    if (far) consider(MX_DIRECT, 1, 4, 16, 64);
+    else if (p.M <= 16 && p.epi != IRIS_EPI_SWIGLU) {
+        /* 16 rows of W per block keep enough blocks in flight without LDS
+         * (6144 x 2560, one row: 4.9 us, 5.4 through LDS); a gate / up group
+         * needs 64 */
+        consider(MX_DIRECT, 1, 1, 16, 16);
+    } else {
+        const int fm = p.M < 64 ? (p.M + 15) / 16 : 4;
+        if (p.M <= 256) consider(MX_ROWS, fm, 4, 16 * fm, 64);
+        if (p.M > 16) {
+            consider(MX_TILE128, 0, 0, 128, 128);
+            if (!mx_exact(p)) consider(MX_TILE256, 0, 0, 256, 256);
         }
     }
-    return q;
+    return best;
 }
 }  // namespace
 
@@ -1403,14 +1448,11 @@ extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_by
     if (plan.kind <= MX_DIRECT) {
         if (f8 ? launch_rows<IRIS_MX_FP8>(P, plan, (unsigned)blocks) : launch_rows<IRIS_MX_FP4>(P, plan, (unsigned)blocks)) return -1;
     } else {
-        /* 16- and 8-bit results are rounded 100 times coarser than what the
-         * single instruction loses; f32 results get f32 sums */
-        const bool exact = f8 && !swiglu && p->epi != IRIS_EPI_BF16;
+        const bool exact = mx_exact(*p);
         const dim3 grid((unsigned)((blocks + 7) / 8 * 8));
 #define MX_T(F, X, T) IRIS_LAUNCH((mx_gemm_tile_kernel<F, X, T, T>), grid, dim3(512), 0, iris_stream(), P)
         if (plan.kind == MX_TILE256) {
             if (!f8) MX_T(IRIS_MX_FP4, false, 256);
-            else if (exact) MX_T(IRIS_MX_FP8, true, 256);
             else MX_T(IRIS_MX_FP8, false, 256);
         } else {
             if (!f8) MX_T(IRIS_MX_FP4, false, 128);
