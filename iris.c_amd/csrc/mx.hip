@@ -470,11 +470,14 @@ template <int V> struct Const {
     static constexpr int value = V;
 };
 
+/* explicit waits stay where they are written, and memory accesses on their side */
 #define WAIT(vm, lgkm)                                              \
     do {                                                            \
+        asm volatile("" ::: "memory");                              \
         __builtin_amdgcn_sched_barrier(0);                          \
         __builtin_amdgcn_s_waitcnt(waitcnt_imm(vm, lgkm));          \
         __builtin_amdgcn_sched_barrier(0);                          \
+        asm volatile("" ::: "memory");                              \
     } while (0)
 
 /* ---- product of few rows ----
@@ -959,9 +962,11 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
             for (int j = 0; j < FN; j++) asm volatile("" ::"v"(acc[i][j]));
     };
     auto barrier = [&]() {
+        asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
     };
     /* Phases between barriers: group 0 runs L(t), C(t) in phases 2t, 2t + 1,
      * group 1 in phases 2t + 1, 2t + 2; L reads step t's fragments, C runs its

@@ -24,6 +24,7 @@
 #include "../../include/iris_qwen3.h"
 #include "../../include/iris_hip.h"
 #include "../../include/iris_synth.h"
+#include "iris_qwen3_model.h"
 #include "iris_st.h"
 
 #include <math.h>
@@ -32,36 +33,6 @@
 #include <string.h>
 
 #define SWIGLU_GROUP 32
-#define HD 128
-
-typedef struct {
-    uint16_t *qkv;       /* [(Hq + 2 Hkv) * 128][h]: Q rows, K rows (head dims permuted), V rows */
-    uint16_t *o;         /* [h][Hq * 128] */
-    uint16_t *gate_up;   /* [2 I][h], gate and up rows interleaved in 32-row groups */
-    uint16_t *down;      /* [h][I] */
-    float *ln1, *ln2;    /* [h] */
-    float *q_norm, *k_norm;   /* [128], permuted like the Q / K rows */
-    iris_mx_t qkv_mx, o_mx, gate_up_mx, down_mx;   /* the same rows in 4 bits, instead (quantized models) */
-} qlayer_t;
-
-struct qwen3_model {
-    int hidden, inter, heads, kv_heads, vocab, layers;
-    float rope_theta;
-    int mode;                 /* 0 Flux, 1 Z-Image */
-    uint16_t *embed;          /* [vocab][h] */
-    qlayer_t *L;
-    /* work buffers for QWEN3_MAX_SEQ_LEN tokens */
-    int *ids;
-    float *x, *out;           /* x [S][h] residual stream; out: the extracted layers, [3][S][h] or [S][3h] */
-    float *host_out;          /* pinned copy of out, one extracted layer after the other; or NULL */
-    uint16_t *a, *qkv, *q, *k, *vt, *attn, *mlp;
-    float *rope_cos, *rope_sin;   /* [S][128], value of pair p at 2p and 2p+1 */
-    float *rp_cos, *rp_sin;       /* [S][64], value of pair p at p (the attention's Q prologue) */
-    float *ws;                    /* split-K partial products */
-    size_t ws_bytes;
-    int quantized;                /* microscaled linears; their inputs: */
-    iris_mx_t a_mx, attn_mx, mlp_mx;
-};
 
 /* position of permuted dim j in the reference's head layout */
 static int head_perm(int j) { return (j & 1) ? (j >> 1) + HD / 2 : (j >> 1); }
@@ -167,32 +138,9 @@ out:
     return rc;
 }
 
-static void mx_free(iris_mx_t *a) {
-    iris_hip_free(a->q);
-    iris_hip_free(a->s);
-    memset(a, 0, sizeof(*a));
-}
-
-static int mx_alloc(iris_mx_t *a, int fmt, size_t rows, int cols) {
-    a->fmt = fmt;
-    a->ld_q = iris_hip_mx_ld_codes(fmt, cols);
-    a->ld_s = iris_hip_mx_ld_scales(cols);
-    a->q = (uint8_t *)iris_hip_malloc(rows * a->ld_q);
-    a->s = (uint8_t *)iris_hip_malloc(rows * a->ld_s);
-    return a->q && a->s ? 0 : -1;
-}
-
-static void free_mx_layers(qwen3_model_t *m) {
-    for (int i = 0; m->L && i < m->layers; i++) {
-        qlayer_t *l = &m->L[i];
-        mx_free(&l->qkv_mx); mx_free(&l->o_mx); mx_free(&l->gate_up_mx); mx_free(&l->down_mx);
-    }
-    mx_free(&m->a_mx); mx_free(&m->attn_mx); mx_free(&m->mlp_mx);
-}
-
 static void free_model(qwen3_model_t *m) {
     if (!m) return;
-    free_mx_layers(m);
+    if (m->mx_free) m->mx_free(m);
     if (m->L) {
         for (int i = 0; i < m->layers; i++) {
             qlayer_t *l = &m->L[i];
@@ -393,35 +341,6 @@ qwen3_model_t *qwen3_model_create_synthetic(int hidden, int intermediate, int he
     return finish(m, &s);
 }
 
-int qwen3_model_quantize(qwen3_model_t *m) {
-    if (!m) return -1;
-    if (m->quantized) return 0;
-    const int h = m->hidden, I = m->inter, qd = m->heads * HD, kd = m->kv_heads * HD, S = QWEN3_MAX_SEQ_LEN;
-    int rc = mx_alloc(&m->a_mx, IRIS_MX_FP8, S, h) || mx_alloc(&m->attn_mx, IRIS_MX_FP8, S, qd) ||
-             mx_alloc(&m->mlp_mx, IRIS_MX_FP8, S, I);
-    for (int i = 0; !rc && i < m->layers; i++) {
-        qlayer_t *l = &m->L[i];
-        rc = mx_alloc(&l->qkv_mx, IRIS_MX_FP4, (size_t)qd + 2 * kd, h) || mx_alloc(&l->o_mx, IRIS_MX_FP4, h, qd) ||
-             mx_alloc(&l->gate_up_mx, IRIS_MX_FP4, 2 * (size_t)I, h) || mx_alloc(&l->down_mx, IRIS_MX_FP4, h, I) ||
-             iris_hip_mx_quantize(&l->qkv_mx, l->qkv, 1, h, qd + 2 * kd, h) ||
-             iris_hip_mx_quantize(&l->o_mx, l->o, 1, qd, h, qd) ||
-             iris_hip_mx_quantize(&l->gate_up_mx, l->gate_up, 1, h, 2 * I, h) ||
-             iris_hip_mx_quantize(&l->down_mx, l->down, 1, I, h, I);
-    }
-    if (iris_hip_sync() || rc) {
-        fail("quantize");
-        free_mx_layers(m);
-        return -1;
-    }
-    for (int i = 0; i < m->layers; i++) {
-        qlayer_t *l = &m->L[i];
-        iris_hip_free(l->qkv); iris_hip_free(l->o); iris_hip_free(l->gate_up); iris_hip_free(l->down);
-        l->qkv = l->o = l->gate_up = l->down = NULL;
-    }
-    m->quantized = 1;
-    return 0;
-}
-
 void qwen3_model_set_extraction_mode(qwen3_model_t *m, int mode) {
     if (m) m->mode = mode ? 1 : 0;
 }
@@ -470,7 +389,7 @@ static int gemm_rms(qwen3_model_t *m, const iris_gemm_problem_t *p, const float 
 }
 
 /* Q, K, V rows of a layer to its attention output */
-static int attend(qwen3_model_t *m, const qlayer_t *l, int S, int n_real) {
+int iris_qwen3_attend(qwen3_model_t *m, const qlayer_t *l, int S, int n_real) {
     const int qd = m->heads * HD, kd = m->kv_heads * HD;
     const int S_pad = (S + 63) / 64 * 64;
     iris_qkprep_args_t q;
@@ -503,7 +422,7 @@ static int layer_forward(qwen3_model_t *m, const qlayer_t *l, const float *next_
     iris_gemm_problem_t p;
     p = prob(m->a, h, l->qkv, h, m->qkv, qd + 2 * kd, S, qd + 2 * kd, h, IRIS_EPI_BF16);
     CK(gemm(m, &p));
-    if (attend(m, l, S, n_real)) return -1;
+    if (iris_qwen3_attend(m, l, S, n_real)) return -1;
     /* o_proj + residual (:461-466, :514-517) */
     p = prob(m->attn, qd, l->o, qd, m->x, h, S, h, qd, IRIS_EPI_GATED_ADD);
     CK(gemm_rms(m, &p, l->ln2, S));
@@ -511,46 +430,6 @@ static int layer_forward(qwen3_model_t *m, const qlayer_t *l, const float *next_
     CK(gemm(m, &p));
     p = prob(m->mlp, I, l->down, I, m->x, h, S, h, I, IRIS_EPI_GATED_ADD);
     CK(gemm_rms(m, &p, next_ln1, S));
-    return 0;
-}
-
-/* residual stream += d (NULL: as it is), then the RMSNorm of it in 8 bits */
-static int mx_rms(qwen3_model_t *m, const uint16_t *d, const float *w, int S) {
-    iris_mx_norm_t a;
-    memset(&a, 0, sizeof(a));
-    a.x = a.x_out = m->x; a.ldx = a.ldxo = m->hidden;
-    a.d = d; a.ldd = m->hidden; a.d_bf16 = 1;
-    a.w = w; a.out = m->a_mx; a.rows = S; a.cols = m->hidden; a.eps = QWEN3_RMS_NORM_EPS;
-    if (!d) a.x_out = NULL;
-    return iris_hip_mx_rmsnorm(&a);
-}
-
-static int mx_gemm(qwen3_model_t *m, const iris_mx_t *A, const iris_mx_t *W, void *out, int ldo, int M, int N, int K, int epi,
-                   const iris_mx_t *mx_out) {
-    iris_mx_gemm_t p;
-    memset(&p, 0, sizeof(p));
-    p.A = *A; p.W = *W; p.out = out; p.ldo = ldo; p.M = M; p.N = N; p.K = K; p.epi = epi;
-    if (mx_out) p.mx_out = *mx_out;
-    return iris_hip_mx_gemm(&p, m->ws, m->ws_bytes);
-}
-
-/* layer_forward of a quantized model: the residual's additions run in the
- * norms that read the stream next; the last layer's, which no norm follows, in
- * its product */
-static int mx_layer_forward(qwen3_model_t *m, const qlayer_t *l, const float *next_ln1, int S, int n_real) {
-    const int h = m->hidden, qd = m->heads * HD, kd = m->kv_heads * HD, I = m->inter;
-    CK(mx_gemm(m, &m->a_mx, &l->qkv_mx, m->qkv, qd + 2 * kd, S, qd + 2 * kd, h, IRIS_EPI_BF16, NULL));
-    if (attend(m, l, S, n_real)) return -1;
-    CK(iris_hip_mx_quantize(&m->attn_mx, m->attn, 1, qd, S, qd));
-    CK(mx_gemm(m, &m->attn_mx, &l->o_mx, m->a, h, S, h, qd, IRIS_EPI_BF16, NULL));
-    CK(mx_rms(m, m->a, l->ln2, S));
-    CK(mx_gemm(m, &m->a_mx, &l->gate_up_mx, NULL, 0, S, 2 * I, h, IRIS_EPI_SWIGLU, &m->mlp_mx));
-    if (!next_ln1) {
-        CK(mx_gemm(m, &m->mlp_mx, &l->down_mx, m->x, h, S, h, I, IRIS_EPI_GATED_ADD, NULL));
-        return 0;
-    }
-    CK(mx_gemm(m, &m->mlp_mx, &l->down_mx, m->a, h, S, h, I, IRIS_EPI_BF16, NULL));
-    CK(mx_rms(m, m->a, next_ln1, S));
     return 0;
 }
 
@@ -604,14 +483,14 @@ float *qwen3_forward(qwen3_model_t *m, const int *input_ids, const int *attentio
     const int beside = m->host_out && slots * n * sizeof(float) >= ((size_t)1 << 20);
     unsigned sent = 0;   /* slots whose download is in flight */
     const iris_norm_args_t first = rms(m, m->L[0].ln1, S);
-    if (m->quantized ? mx_rms(m, NULL, m->L[0].ln1, S) : iris_hip_rownorm(&first)) {
+    if (m->mx_first ? m->mx_first(m, S) : iris_hip_rownorm(&first)) {
         fail("input norm");
         return NULL;
     }
     for (int i = 0; i <= last; i++) {
         const float *next_ln1 = i < last ? m->L[i + 1].ln1 : NULL;
-        if (m->quantized ? mx_layer_forward(m, &m->L[i], next_ln1, S, n_real)
-                         : layer_forward(m, &m->L[i], next_ln1, S, n_real)) {
+        if (m->mx_layer ? m->mx_layer(m, &m->L[i], next_ln1, S, n_real)
+                        : layer_forward(m, &m->L[i], next_ln1, S, n_real)) {
             finish_downloads(sent);
             return NULL;
         }
