@@ -1358,7 +1358,7 @@ bool mx_exact(const iris_mx_gemm_t &p) {
     return p.A.fmt == IRIS_MX_FP8 && p.epi != IRIS_EPI_SWIGLU && p.epi != IRIS_EPI_BF16;
 }
 
-MxPlan mx_plan(const iris_mx_gemm_t &p, int steps, size_t ws_bytes) {
+MxPlan mx_plan(const iris_mx_gemm_t &p, int steps, size_t ws_bytes, double *estimate) {
     const int cus = iris_cu_count() > 0 ? iris_cu_count() : 1;
     /* the staging kernels reach rows by 32-bit offsets */
     long long ld = p.A.ld_q;
@@ -1414,26 +1414,33 @@ MxPlan mx_plan(const iris_mx_gemm_t &p, int steps, size_t ws_bytes) {
             if (!mx_exact(p)) consider(MX_TILE256, 0, 0, 256, 256);
         }
     }
+    *estimate = least;
     return best;
 }
-}  // namespace
 
-extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_bytes) {
-    if (!p) return iris_set_error("mx_gemm: null problem");
-    if (p->M <= 0 || p->N <= 0) return 0;
-    if (p->K <= 0) return iris_set_error("mx_gemm: K %d", p->K);
-    if (check_mx("mx_gemm A", p->A, p->K) || check_mx("mx_gemm W", p->W, p->K)) return -1;
-    if (p->W.fmt != IRIS_MX_FP4) return iris_set_error("mx_gemm: weights of format %d, not IRIS_MX_FP4", p->W.fmt);
+/* Rows of A for a launch of their own: as many as fill whole rounds of 256 x
+ * 256 tiles, where those behind them, planned by themselves, take less than
+ * their part of a last round (4608 x 3840 x 10240 e2m1, 270 tiles for 256 CUs:
+ * 132 -> 110 us). 0: one launch. */
+int mx_main_rows(const iris_mx_gemm_t &p, int steps, size_t ws_bytes, double whole) {
+    const int cus = iris_cu_count() > 0 ? iris_cu_count() : 1;
+    const int tm = (p.M + 255) / 256, tn = (p.N + 255) / 256;
+    const long long rounds = (long long)tm * tn / cus;
+    if (mx_exact(p) || rounds < 1 || rounds * cus < tn) return 0;
+    const int rows = (int)(rounds * cus / tn) * 256;
+    if (rows >= p.M) return 0;
+    iris_mx_gemm_t part = p;
+    double us[2];
+    part.M = rows;
+    (void)mx_plan(part, steps, ws_bytes, &us[0]);
+    part.M = p.M - rows;
+    (void)mx_plan(part, steps, ws_bytes, &us[1]);
+    return us[0] + us[1] < 0.95 * whole ? rows : 0;
+}
+/* a checked problem; ws_bytes 0: no workspace */
+int mx_run(const iris_mx_gemm_t *p, float *ws, size_t ws_bytes) {
     const bool swiglu = p->epi == IRIS_EPI_SWIGLU, mx = swiglu && p->mx_out.q;
-    if (!swiglu && p->epi != IRIS_EPI_F32 && p->epi != IRIS_EPI_BF16 && p->epi != IRIS_EPI_GATED_ADD &&
-        p->epi != IRIS_EPI_ADD)
-        return iris_set_error("mx_gemm: epilogue %d", p->epi);
-    if (swiglu && (p->N % 64 || p->vec)) return iris_set_error("mx_gemm: SWIGLU needs N %% 64 == 0 (%d) and no vec", p->N);
-    if (!swiglu && p->mx_out.q) return iris_set_error("mx_gemm: mx_out is for SWIGLU");
     const int nout = swiglu ? p->N / 2 : p->N;
-    if (mx ? check_mx("mx_gemm output", p->mx_out, nout) : !p->out ? iris_set_error("mx_gemm: null output") : 0) return -1;
-    if (!mx && p->ldo < nout) return iris_set_error("mx_gemm: output row stride %d of %d columns", p->ldo, nout);
-    if (!iris_hip_available()) return -1;
     MxGemm P;
     P.aq = p->A.q; P.as = p->A.s; P.lda = p->A.ld_q; P.ldas = p->A.ld_s;
     P.wq = p->W.q; P.ws = p->W.s; P.ldw = p->W.ld_q; P.ldws = p->W.ld_s;
@@ -1441,7 +1448,21 @@ extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_by
     P.steps = pad_to(p->K, 128) / 128;
     P.oq = mx ? p->mx_out.q : nullptr; P.os = p->mx_out.s;
     P.ldoq = p->mx_out.ld_q; P.ldos = p->mx_out.ld_s; P.ofmt = p->mx_out.fmt;
-    const MxPlan plan = mx_plan(*p, P.steps, ((uintptr_t)ws & 15) || !ws ? 0 : ws_bytes);
+    double whole;
+    const MxPlan plan = mx_plan(*p, P.steps, ws_bytes, &whole);
+    if (const int rows = mx_main_rows(*p, P.steps, ws_bytes, whole)) {
+        iris_mx_gemm_t part = *p;
+        part.M = rows;
+        if (mx_run(&part, ws, ws_bytes)) return -1;
+        part.M = p->M - rows;
+        part.A.q += (size_t)rows * p->A.ld_q;
+        part.A.s += (size_t)rows * p->A.ld_s;
+        if (mx) {
+            part.mx_out.q += (size_t)rows * p->mx_out.ld_q;
+            part.mx_out.s += (size_t)rows * p->mx_out.ld_s;
+        } else part.out = (char *)p->out + (size_t)rows * p->ldo * (swiglu || p->epi == IRIS_EPI_BF16 ? 2 : 4);
+        return mx_run(&part, ws, ws_bytes);
+    }
     P.tiles_m = plan.tiles_m; P.tiles_n = plan.tiles_n; P.chunks = plan.chunks; P.per_chunk = plan.per_chunk;
     const long long blocks = (long long)plan.tiles_m * plan.tiles_n * plan.chunks;
     if (blocks > 0x7fffffff / 2) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
@@ -1474,4 +1495,24 @@ extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_by
         return iris_launch_check("mx_reduce_kernel");
     }
     return 0;
+}
+}  // namespace
+
+extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_bytes) {
+    if (!p) return iris_set_error("mx_gemm: null problem");
+    if (p->M <= 0 || p->N <= 0) return 0;
+    if (p->K <= 0) return iris_set_error("mx_gemm: K %d", p->K);
+    if (check_mx("mx_gemm A", p->A, p->K) || check_mx("mx_gemm W", p->W, p->K)) return -1;
+    if (p->W.fmt != IRIS_MX_FP4) return iris_set_error("mx_gemm: weights of format %d, not IRIS_MX_FP4", p->W.fmt);
+    const bool swiglu = p->epi == IRIS_EPI_SWIGLU, mx = swiglu && p->mx_out.q;
+    if (!swiglu && p->epi != IRIS_EPI_F32 && p->epi != IRIS_EPI_BF16 && p->epi != IRIS_EPI_GATED_ADD &&
+        p->epi != IRIS_EPI_ADD)
+        return iris_set_error("mx_gemm: epilogue %d", p->epi);
+    if (swiglu && (p->N % 64 || p->vec)) return iris_set_error("mx_gemm: SWIGLU needs N %% 64 == 0 (%d) and no vec", p->N);
+    if (!swiglu && p->mx_out.q) return iris_set_error("mx_gemm: mx_out is for SWIGLU");
+    const int nout = swiglu ? p->N / 2 : p->N;
+    if (mx ? check_mx("mx_gemm output", p->mx_out, nout) : !p->out ? iris_set_error("mx_gemm: null output") : 0) return -1;
+    if (!mx && p->ldo < nout) return iris_set_error("mx_gemm: output row stride %d of %d columns", p->ldo, nout);
+    if (!iris_hip_available()) return -1;
+    return mx_run(p, ws, ((uintptr_t)ws & 15) || !ws ? 0 : ws_bytes);
 }
