@@ -363,6 +363,42 @@ def test_gemm_large_tiles_swiglu(lib, ws, M, N, K, afmt, mx_fmt):
     p.close()
 
 
+@pytest.mark.parametrize("afmt,epi,mx_fmt", [(FP8, EPI_BF16, None), (FP4, EPI_F32, None), (FP8, EPI_SWIGLU, FP8),
+                                             (FP4, EPI_SWIGLU, None)])
+def test_gemm_rows_behind_whole_rounds(lib, ws, afmt, epi, mx_fmt):
+    """More than 256 tiles of 256 x 256: whole rounds, and the rows behind them by themselves."""
+    p = Product(4400, 4160, 2000, afmt, epi, pad=1, mx_fmt=mx_fmt)
+    assert len(kernels(lib, lambda: p.check(p.run(lib, ws.ptr)))) >= 2
+    p.close()
+
+
+def kernels(lib, call):
+    """The (kernel, blocks) pairs that a call launches."""
+    lib.iris_hip_profile_read.argtypes = [ctypes.c_void_p, ctypes.c_int]
+    assert lib.iris_hip_profile_enable(1) == 0
+    call()
+    rec = (tl.KernelTime * 64)()
+    n = lib.iris_hip_profile_read(ctypes.byref(rec), 64)
+    assert lib.iris_hip_profile_enable(0) == 0
+    return [(r.kernel.decode(), r.grid) for r in rec[:n]]
+
+
+@pytest.mark.parametrize("M,N,K,afmt,epi,want", [
+    (1, 320, 1000, FP8, EPI_F32, "direct_kernel<AF, 1, 1>"), (16, 64, 5000, FP4, EPI_BF16, "direct_kernel<AF, 1, 1>"),
+    (5, 128, 9000, FP8, EPI_SWIGLU, "rows_kernel<AF, FM, FN>"),
+    (20, 320, 9000, FP4, EPI_F32, "rows_kernel<AF, FM, FN>"), (40, 320, 9000, FP8, EPI_BF16, "rows_kernel<AF, FM, FN>"),
+    (64, 320, 9000, FP8, EPI_BF16, "rows_kernel<AF, FM, FN>"), (64, 320, 9000, FP8, EPI_BF16, "mx_reduce_kernel"),
+    (500, 2000, 640, FP8, EPI_F32, "tile_kernel<0, 1, 128, 128>"), (500, 2000, 640, FP8, EPI_BF16, "tile_kernel<0, 0, 128, 128>"),
+    (500, 2000, 640, FP4, EPI_F32, "tile_kernel<1, 0, 128, 128>"), (4096, 4096, 512, FP8, EPI_BF16, "tile_kernel<0, 0, 256, 256>"),
+    (4096, 4096, 512, FP4, EPI_F32, "tile_kernel<1, 0, 256, 256>")])
+def test_every_kernel_is_reached(lib, ws, M, N, K, afmt, epi, want):
+    p = Product(M, N, K, afmt, epi)
+    names = [k for k, _ in kernels(lib, lambda: p.check(p.run(lib, ws.ptr)))]
+    flat = " ".join(names).replace("IRIS_MX_FP8", "0").replace("IRIS_MX_FP4", "1").replace("false", "0").replace("true", "1")
+    assert want in flat, flat
+    p.close()
+
+
 @pytest.mark.parametrize("M,N,K", [(3, 70, 200), (300, 600, 640), (37, 512, 4096)])
 @pytest.mark.parametrize("afmt", [FP8, FP4])
 def test_gemm_nan_blocks(lib, ws, M, N, K, afmt):
