@@ -214,11 +214,11 @@ template <int DT> __device__ __forceinline__ Row8 norm_row8(const NormParams &P,
     return x;
 }
 
-/* DT: 0 no d, 1 f32, 2 bf16. One block per row, R chunks of 8 columns a
- * thread held in registers; R 0: any length, the row read twice (the second
+/* DT: 0 no d, 1 f32, 2 bf16. One block of TH threads per row, R chunks of 8
+ * columns a thread held in registers; R 0: any length, the row read twice (the second
  * time from x_out where there is a d: the thread's own stores). */
-template <int FMT, int DT, int R> __global__ __launch_bounds__(NT) void mx_rmsnorm_kernel(const NormParams P) {
-    __shared__ double red[NT / IRIS_WAVE];
+template <int FMT, int DT, int TH, int R> __global__ __launch_bounds__(TH) void mx_rmsnorm_kernel(const NormParams P) {
+    __shared__ double red[TH / IRIS_WAVE];
     const size_t row = blockIdx.x;
     Row8 t[R ? R : 1];
     double ss = 0.0;
@@ -229,14 +229,14 @@ template <int FMT, int DT, int R> __global__ __launch_bounds__(NT) void mx_rmsno
     if constexpr (R > 0) {
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const int c = (r * NT + (int)threadIdx.x) * 8;
+            const int c = (r * TH + (int)threadIdx.x) * 8;
             if (c < P.cols_pad) {
                 t[r] = norm_row8<DT>(P, row, c, true);
                 square(t[r]);
             }
         }
     } else {
-        for (int c = (int)threadIdx.x * 8; c < P.cols_pad; c += NT * 8) square(norm_row8<DT>(P, row, c, true));
+        for (int c = (int)threadIdx.x * 8; c < P.cols_pad; c += TH * 8) square(norm_row8<DT>(P, row, c, true));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
@@ -244,7 +244,7 @@ template <int FMT, int DT, int R> __global__ __launch_bounds__(NT) void mx_rmsno
     __syncthreads();
     ss = 0.0;
 #pragma unroll
-    for (int i = 0; i < NT / IRIS_WAVE; i++) ss += red[i];
+    for (int i = 0; i < TH / IRIS_WAVE; i++) ss += red[i];
     const double inv = 1.0 / sqrt(ss / P.cols + (double)P.eps);
     auto put = [&](const Row8 &x, int c) {
         const Row8 w = load8<false>(P.w, c, P.cols, P.vw);   /* zeros past the row's end */
@@ -264,7 +264,7 @@ template <int FMT, int DT, int R> __global__ __launch_bounds__(NT) void mx_rmsno
     if constexpr (R > 0) {
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const int c = (r * NT + (int)threadIdx.x) * 8;
+            const int c = (r * TH + (int)threadIdx.x) * 8;
             if (c < P.cols_pad) put(t[r], c);
         }
     } else {
@@ -274,7 +274,7 @@ template <int FMT, int DT, int R> __global__ __launch_bounds__(NT) void mx_rmsno
             P2.ldx = P.ldxo;
             P2.vx = P.vo;
         }
-        for (int c = (int)threadIdx.x * 8; c < P.cols_pad; c += NT * 8) put(norm_row8<0>(P2, row, c, false), c);
+        for (int c = (int)threadIdx.x * 8; c < P.cols_pad; c += TH * 8) put(norm_row8<0>(P2, row, c, false), c);
     }
 }
 
@@ -1248,13 +1248,21 @@ int iris_hip_mx_dequantize(void *y, int is_bf16, int ldy, const iris_mx_t *a, in
 }  /* extern "C" */
 
 namespace {
+/* Threads per row, us (rows that no cache holds; 128 / 256 / 512): 20000 x 320
+ * 19.9 / 25.9 / 42.4; 512 x 2560 6.8 / 6.0 / 5.5; 8192 x 2160 50.7 / 48.3 /
+ * 49.7; 4608 x 3840 50.8 / 45.5 / 44.1 (4.4 TB/s); 1000 x 10240 36.5 / 34.3 /
+ * 25.9 */
 template <int FMT, int DT> void launch_norm(const NormParams &P, int rows) {
-    const int r = (P.cols_pad / 8 + NT - 1) / NT;
-#define MX_N(R) IRIS_LAUNCH((mx_rmsnorm_kernel<FMT, DT, R>), dim3(rows), dim3(NT), 0, iris_stream(), P)
-    if (r == 1) MX_N(1);
-    else if (r == 2) MX_N(2);
-    else if (r <= 4) MX_N(4);
-    else MX_N(0);
+    const int lanes = P.cols_pad / 8;
+#define MX_N(TH, R) IRIS_LAUNCH((mx_rmsnorm_kernel<FMT, DT, TH, R>), dim3(rows), dim3(TH), 0, iris_stream(), P)
+    if (lanes <= 64) MX_N(64, 1);
+    else if (lanes <= 128) MX_N(128, 1);
+    else if (lanes <= 256) MX_N(256, 1);
+    else if (lanes <= 384 && rows >= 1024) MX_N(256, 2);
+    else if (lanes <= 512) MX_N(512, 1);
+    else if (lanes <= 1024) MX_N(512, 2);
+    else if (lanes <= 2048) MX_N(512, 4);
+    else MX_N(512, 0);
 #undef MX_N
 }
 }  // namespace

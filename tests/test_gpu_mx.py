@@ -155,7 +155,7 @@ def norm_reference(x, d, gate, w, scale, eps):
 
 
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 33), (2, 128), (5, 2047), (37, 2048), (4, 2049), (2, 2560), (9, 3840),
-                                       (2, 4104), (3, 8192), (2, 8193), (1, 20000)])
+                                       (2, 4104), (3, 8192), (2, 8193), (1, 20000), (4, 500), (4, 1000), (1100, 2100)])
 @pytest.mark.parametrize("fmt", [FP8, FP4])
 @pytest.mark.parametrize("add", ["none", "f32", "bf16"])
 def test_rmsnorm(lib, rows, cols, fmt, add):
