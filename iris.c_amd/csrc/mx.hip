@@ -480,6 +480,20 @@ template <int V> struct Const {
         asm volatile("" ::: "memory");                              \
     } while (0)
 
+/* part[0] + part[stride] + .. of n waves, in order; 4 reads in flight */
+__device__ __forceinline__ f32x4 mx_sum_waves(const f32x4 *part, int stride, int n) {
+    f32x4 s = part[0];
+    for (int w = 1; w < n; w += 4) {
+        f32x4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = part[min(w + k, n - 1) * stride];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (w + k < n) s += v[k];
+    }
+    return s;
+}
+
 /* ---- product of few rows ----
  * Bound by W's bytes and by the number of 128-byte lines that loads touch (1.5
  * ns each and CU), not by the matrix instructions. A block's waves share 16 FM
@@ -617,11 +631,7 @@ __global__ __launch_bounds__((64 * RowsShape<AF, FM, FN>::WAVES)) void mx_gemm_r
 #pragma unroll
         for (int j = 0; j < FN; j++) part[(wave * FM * FN + i * FN + j) * 64 + lane] = acc[i][j];
     __syncthreads();
-    auto sum = [&](int i, int j) {
-        f32x4 s = part[(i * FN + j) * 64 + lane];
-        for (int w = 1; w < waves; w++) s += part[(w * FM * FN + i * FN + j) * 64 + lane];
-        return s;
-    };
+    auto sum = [&](int i, int j) { return mx_sum_waves(part + (i * FN + j) * 64 + lane, FM * FN * 64, waves); };
     const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
     if constexpr (FN == 4) {
         if (P.epi == IRIS_EPI_SWIGLU) {
@@ -716,11 +726,7 @@ template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm
 #pragma unroll
         for (int j = 0; j < FN; j++) part[(wave * FM * FN + i * FN + j) * 64 + lane] = acc[i][j];
     __syncthreads();
-    auto sum = [&](int i, int j) {
-        f32x4 s = part[(i * FN + j) * 64 + lane];
-        for (int w = 1; w < waves; w++) s += part[(w * FM * FN + i * FN + j) * 64 + lane];
-        return s;
-    };
+    auto sum = [&](int i, int j) { return mx_sum_waves(part + (i * FN + j) * 64 + lane, FM * FN * 64, waves); };
     const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
     if constexpr (FN == 4) {
         if (P.epi == IRIS_EPI_SWIGLU) {
@@ -748,11 +754,17 @@ __global__ __launch_bounds__(NT) void mx_reduce_kernel(const MxGemm P, const flo
     const size_t stride = (size_t)P.M * P.N;
     const bool vec = (P.N & 3) == 0 && ((uintptr_t)part & 15) == 0;
     auto sum8 = [&](int col) {
-        Row8 s = load8<false>(part + (size_t)m * P.N, col, P.N, vec);
-        for (int k = 1; k < P.chunks; k++) {
-            const Row8 x = load8<false>(part + k * stride + (size_t)m * P.N, col, P.N, vec);
+        const float *row = part + (size_t)m * P.N;
+        Row8 s = load8<false>(row, col, P.N, vec);
+        for (int k = 1; k < P.chunks; k += 3) {   /* 3 chunks' loads in flight */
+            Row8 x[3];
 #pragma unroll
-            for (int j = 0; j < 8; j++) s.v[j] += x.v[j];
+            for (int i = 0; i < 3; i++) x[i] = load8<false>(row + min(k + i, P.chunks - 1) * stride, col, P.N, vec);
+#pragma unroll
+            for (int i = 0; i < 3; i++)
+                if (k + i < P.chunks)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) s.v[j] += x[i].v[j];
         }
         return s;
     };
@@ -1312,8 +1324,15 @@ template <int AF, int FM, int FN> int launch_rows_of(const MxGemm &P, unsigned b
     using Sh = RowsShape<AF, FM, FN>;
     /* units of 256 columns, as evenly as the waves that LDS holds take them */
     const int most = (int)blocks <= iris_cu_count() ? Sh::WAVES : Sh::WAVES2;
-    const int units = (P.per_chunk + 1) / 2, rounds = (units + most - 1) / most;
-    const int waves = (units + rounds - 1) / rounds;
+    const int units = (P.per_chunk + 1) / 2;
+    /* rounds of a unit per wave: its loads, about two units' instructions, and
+     * the instructions of the SIMD with the most waves */
+    int waves = 1;
+    for (int w = 2, least = 3 * units; w <= most && w <= units; w++) {
+        const int full = units / w, rest = units % w;
+        const int cost = 2 * (full + (rest > 0)) + full * ((w + 3) / 4) + (rest + 3) / 4;
+        if (cost < least) least = cost, waves = w;
+    }
     const int smem = Sh::SCALES + waves * Sh::UNIT;
     static_assert(Sh::UNIT >= FM * FN * 1024, "the sums fit where the units were");
     static std::once_flag once;
