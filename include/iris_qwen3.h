@@ -68,9 +68,9 @@ qwen3_model_t *qwen3_model_create_synthetic(int hidden, int intermediate, int he
  * are then microscaled 8-bit rows, written by the residual RMSNorm and by the
  * SwiGLU product, or quantised from the attention's output. Embedding, norms,
  * attention and the residual stream stay as they are. 3.8 times less weight
- * memory and traffic; an activation is rounded by at most 2^-4 of its value, a
- * weight by at most 2^-2. Returns 0, or -1 with a message, the model then
- * unchanged. */
+ * memory and traffic; an activation moves by at most 2^-3 and a weight by at
+ * most 2^-2 of the largest magnitude among its 32 columns. Returns 0, or -1
+ * with a message, the model then unchanged. */
 int qwen3_model_quantize(qwen3_model_t *model);
 
 #ifdef __cplusplus

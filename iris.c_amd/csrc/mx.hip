@@ -98,7 +98,9 @@ template <bool BF16> __device__ __forceinline__ Row8 load8(const void *row, int 
 }
 
 /* One lane per 8 columns, rows one after the other (cpr = padded columns / 8
- * lanes each, a multiple of 16, so a quad stays in its block). */
+ * lanes each, a multiple of 16, so a quad stays in its block). Bound by the
+ * bytes: 19456 x 2560 bf16 to e2m1 27.5 us, 4.6 TB/s; 512 x 4096 bf16 to e4m3
+ * 3.4 us, a launch. */
 template <int FMT, bool BF16>
 __global__ __launch_bounds__(NT) void mx_quantize_kernel(uint8_t *q, uint8_t *s, int ld_q, int ld_s, const void *x,
                                                          int ldx, int cols, uint32_t cpr, uint32_t n, bool vec) {
@@ -115,6 +117,7 @@ __device__ __forceinline__ float mx_two(int s) {
     return s == 255 ? __int_as_float(0x7fc00000) : s ? __int_as_float(s << 23) : __int_as_float(0x00400000);
 }
 
+/* 19456 x 2560 e2m1 to bf16: 21.0 us, 6.0 TB/s (the codes from the caches). */
 template <int FMT, bool BF16>
 __global__ __launch_bounds__(NT) void mx_dequantize_kernel(void *y, int ldy, const uint8_t *q, const uint8_t *s,
                                                            int ld_q, int ld_s, int cols, uint32_t cpr, uint32_t n,
@@ -214,7 +217,9 @@ template <int DT> __device__ __forceinline__ Row8 norm_row8(const NormParams &P,
     return x;
 }
 
-/* DT: 0 no d, 1 f32, 2 bf16. One block of TH threads per row, R chunks of 8
+/* Bound by the bytes, one pass over them: 4608 x 3840, bf16 d and gate, 42.5 us
+ * (4.6 TB/s); 512 x 2560, f32 d, 5.7 us; one row 4.6 us, a launch.
+ * DT: 0 no d, 1 f32, 2 bf16. One block of TH threads per row, R chunks of 8
  * columns a thread held in registers; R 0: any length, the row read twice (the second
  * time from x_out where there is a d: the thread's own stores). */
 template <int FMT, int DT, int TH, int R> __global__ __launch_bounds__(TH) void mx_rmsnorm_kernel(const NormParams P) {
@@ -503,7 +508,11 @@ __device__ __forceinline__ f32x4 mx_sum_waves(const f32x4 *part, int stride, int
  * the unit before is multiplied. Fragments straight from global memory touch
  * each line twice, and a wave's loads in registers leave room for half the
  * waves: gate and up of 37 rows 24.8 us. Scales of 4096 columns are loaded by
- * the whole block, a line a row. The waves' sums are added in wave order. */
+ * the whole block, a line a row. The waves' sums are added in wave order.
+ * Measured, e4m3 A: 37 x 19456 x 2560 with SwiGLU 14.3 us (26.5 MB of W at 1.9
+ * TB/s; of a block's 10 us a third is launch, first loads and scales, a third
+ * instructions, a third sums and epilogue), 37 x 6144 x 2560 8.6; e2m1 A: 37 x
+ * 11520 x 3840 7.3 (3.2 TB/s). */
 template <int AF, int FM, int FN> struct RowsShape {
     static constexpr int A_ROW = AF == IRIS_MX_FP8 ? 256 : 128;    /* bytes of 256 columns */
     static constexpr int A_BYTES = FM * 16 * A_ROW, UNIT = A_BYTES + FN * 2048;
@@ -652,7 +661,8 @@ __global__ __launch_bounds__((64 * RowsShape<AF, FM, FN>::WAVES)) void mx_gemm_r
  * of 512 columns in turn: for one to 16 rows of A (plain epilogues), and for
  * rows further apart than the other kernels' 32-bit offsets reach. Whole
  * 128-byte lines of the codes and one 16-byte load of scales a row for 4
- * steps (a 4-byte load per step touched as many lines as W). */
+ * steps (a 4-byte load per step touched as many lines as W). One row x 6144 x
+ * 2560: 4.5 us, of which 3 are the launch; W's 8.4 MB at 1.9 TB/s. */
 template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm_direct_kernel(MxGemm P) {
     extern __shared__ f32x4 part[];   /* [waves][FM * FN tiles][64 lanes] */
     const int tiles = P.tiles_m * P.tiles_n;
@@ -744,7 +754,8 @@ template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm
 
 /* ---- sums of a split product ----
  * One lane per 8 output columns: the chunks' partial sums in order, then the
- * epilogue. */
+ * epilogue. 512 x 2560 of 3 chunks: 7.6 us, 5 where they are still in the
+ * caches (4 TB/s). */
 __global__ __launch_bounds__(NT) void mx_reduce_kernel(const MxGemm P, const float *part, uint32_t n, uint32_t cpr) {
     const uint32_t i = blockIdx.x * NT + threadIdx.x;
     if (i >= n) return;
@@ -815,7 +826,17 @@ __global__ __launch_bounds__(NT) void mx_reduce_kernel(const MxGemm P, const flo
  * Scales: 16 bytes of a row are 512 columns. They are loaded into LDS as they
  * are, then a lane transposes the 4 x 4 bytes of a row so that the bytes of
  * lane group g (block g of each 128 columns) make one word; a fragment's lane
- * reads its word once per 512 columns and shifts it by a byte per 128. */
+ * reads its word once per 512 columns and shifts it by a byte per 128.
+ * Measured on 256 x 256 tiles: e4m3 A, 4608 x 20480 x 3840 with SwiGLU 263 us,
+ * 2.75 PFLOP/s: 2620 cycles per K step, of which the matrix instructions are
+ * 2110, at 1.8 to 2.1 GHz, the clock that such a kernel is given. e2m1 A, 4352
+ * x 3840 x 10240 86.6 us, 3.95 PFLOP/s: 3310 cycles per 256 columns, the
+ * instructions 2050; reading a step's fragments beside the loads into LDS takes
+ * 1500 of a phase's 1650. 128 x 128 tiles, f32 sums: 512 x 2560 x 9728 in 3
+ * ranges 33.0 us and their sum; A's two parts double the instructions. 4 waves
+ * of 128 x 128 each would read a third less from LDS; their 256 sums a lane fill
+ * one half of the registers, and the compiler keeps the operands of the other
+ * half in scratch memory. */
 __device__ __forceinline__ bool rows16_ok(const void *p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0; }
 
 template <int AF, bool SPLIT, int BM, int BN>
@@ -1323,6 +1344,8 @@ struct MxPlan {
 template <int AF, int FM, int FN> int launch_rows_of(const MxGemm &P, unsigned blocks) {
     using Sh = RowsShape<AF, FM, FN>;
     /* units of 256 columns, as evenly as the waves that LDS holds take them */
+    /* two blocks on a CU where there are more than CUs: 37 x 19456 x 2560, 304
+     * blocks, 17.0 us, 21.8 with one block of all waves */
     const int most = (int)blocks <= iris_cu_count() ? Sh::WAVES : Sh::WAVES2;
     const int units = (P.per_chunk + 1) / 2;
     /* rounds of a unit per wave: its loads, about two units' instructions, and
@@ -1368,8 +1391,8 @@ template <int AF> int launch_rows(const MxGemm &P, const MxPlan &plan, unsigned 
  * split's partial sums and their second launch are 3 and their bytes at 4 TB/s.
  * Measured, us: 300 x 19456 x 2560 e4m3 to bf16: 24.1 on 128 x 128 tiles, 31.6
  * on 256 x 256; 512 rows 32.7 and 28.7; 512 x 2560 x 9728 to f32: 63 unsplit,
- * 36.6 in 3 ranges; 64 x 6144 x 2560: 12.8 through mx_gemm_rows_kernel, 14.4
- * on tiles; 64 x 19456 x 2560: 22.2 and 16.2. */
+ * 36.6 in 3 ranges; 64 x 6144 x 2560: 10.7 through mx_gemm_rows_kernel, 15.1
+ * on tiles; 64 x 19456 x 2560: 22.1 and 15.5. */
 template <int AF> void rows_waves(int fm, int *one, int *two) {
     switch (fm) {
     case 1: *one = RowsShape<AF, 1, 4>::WAVES; *two = RowsShape<AF, 1, 4>::WAVES2; break;
