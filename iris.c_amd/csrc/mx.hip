@@ -1106,14 +1106,14 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
     }
     WAIT(0, 0);   /* no load outstanding at exit */
     const int lane = hidden_lane(), lr = lane & 15, lg = lane >> 4;
-    /* Whole tiles of 16-bit or microscaled output leave through LDS, two of a
-     * wave's 16-row tiles at a time, so that a row's part of a wave (256, 128
-     * or 64 bytes) is written by neighbouring lanes: 8-byte stores of 16 rows
-     * each took 10 us more of 4096 x 4096 x 2560. */
-    const bool full = m0 + BM <= P.M && n0 + BN <= P.N;
+    /* 16-bit output leaves through LDS, two of a wave's 16-row tiles at a time,
+     * so that a row's part of a wave (256, 128 or 64 bytes) is written by
+     * neighbouring lanes: 8-byte stores of 16 rows each took 10 us more of 4096
+     * x 4096 x 2560, and of 1227 x 11520 x 3840, of whose tiles a fifth are cut,
+     * 42.7 us rather than 35.5. */
     uint8_t *const st = lds + wave * 8192;
     static_assert(sizeof(lds) >= 8 * 8192, "a wave's part");
-    if (full && P.epi == IRIS_EPI_BF16 && rows16_ok(P.out, P.ldo)) {
+    if (P.epi == IRIS_EPI_BF16 && rows16_ok(P.out, P.ldo)) {
         __syncthreads();   /* every wave is done with the stages */
 #pragma unroll
         for (int ip = 0; ip < FM; ip += 2) {
@@ -1122,7 +1122,10 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
                 float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 if (P.vec)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) v[r] = P.vec[n0 + wn * TWN + j * 16 + 4 * lg + r];
+                    for (int r = 0; r < 4; r++) {
+                        const int n = n0 + wn * TWN + j * 16 + 4 * lg + r;
+                        v[r] = n < P.N ? P.vec[n] : 0.0f;
+                    }
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const f32x4 x = acc[ip + i][j];
@@ -1132,17 +1135,24 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
                                    (uint32_t)f2bf_hw(x[2] + v[2]) | (uint32_t)f2bf_hw(x[3] + v[3]) << 16);
                 }
             }
-            uint16_t *const out = (uint16_t *)P.out + (size_t)(m0 + wm * TWM + ip * 16) * P.ldo + n0 + wn * TWN;
+            const int m = m0 + wm * TWM + ip * 16, n = n0 + wn * TWN;
             constexpr int CPR = FN * 2;
 #pragma unroll
             for (int k = 0; k < 32 * CPR / 64; k++) {
-                const int c = k * 64 + lane, row = c / CPR, ch = c % CPR;
-                *(u32x4 *)(out + (size_t)row * P.ldo + ch * 8) = *(const u32x4 *)(st + row * (TWN * 2) + ((ch ^ (row & (CPR - 1))) << 4));
+                const int c = k * 64 + lane, row = c / CPR, ch = c % CPR, col = n + ch * 8;
+                const u32x4 x = *(const u32x4 *)(st + row * (TWN * 2) + ((ch ^ (row & (CPR - 1))) << 4));
+                uint16_t *const out = (uint16_t *)P.out + (size_t)(m + row) * P.ldo + col;
+                if (m + row >= P.M) continue;
+                if (col + 8 <= P.N) *(u32x4 *)out = x;
+                else
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (col + j < P.N) out[j] = (uint16_t)(x[j >> 1] >> (16 * (j & 1)));
             }
         }
         return;
     }
-    if (full && P.epi == IRIS_EPI_SWIGLU && !P.oq && rows16_ok(P.out, P.ldo)) {
+    if (P.epi == IRIS_EPI_SWIGLU && !P.oq && rows16_ok(P.out, P.ldo)) {
         __syncthreads();
 #pragma unroll
         for (int ip = 0; ip < FM; ip += 2) {
@@ -1160,12 +1170,14 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
                         *(uint2 *)(st + row * TWN + (((4 * j + 2 * h + (lg >> 1)) ^ (row & (FN - 1))) << 4) + (lg & 1) * 8) =
                             make_uint2((uint32_t)y[0] | (uint32_t)y[1] << 16, (uint32_t)y[2] | (uint32_t)y[3] << 16);
                     }
-            uint16_t *const out = (uint16_t *)P.out + (size_t)(m0 + wm * TWM + ip * 16) * P.ldo + (n0 + wn * TWN) / 2;
+            const int m = m0 + wm * TWM + ip * 16, n = (n0 + wn * TWN) / 2;
             constexpr int CPR = FN;
 #pragma unroll
             for (int k = 0; k < 32 * CPR / 64; k++) {
-                const int c = k * 64 + lane, row = c / CPR, ch = c % CPR;
-                *(u32x4 *)(out + (size_t)row * P.ldo + ch * 8) = *(const u32x4 *)(st + row * TWN + ((ch ^ (row & (CPR - 1))) << 4));
+                const int c = k * 64 + lane, row = c / CPR, ch = c % CPR, col = n + ch * 8;
+                const u32x4 x = *(const u32x4 *)(st + row * TWN + ((ch ^ (row & (CPR - 1))) << 4));
+                /* N / 2 is a multiple of 32: 8 columns are inside or none */
+                if (m + row < P.M && col < P.N / 2) *(u32x4 *)((uint16_t *)P.out + (size_t)(m + row) * P.ldo + col) = x;
             }
         }
         return;

@@ -354,6 +354,24 @@ def test_gemm_large_tiles(lib, ws, M, N, K, afmt, epi):
     p.close()
 
 
+@pytest.mark.parametrize("M,N,K,epi", [(301, 1349, 640, EPI_BF16), (2113, 4005, 200, EPI_BF16), (301, 1344, 640, EPI_SWIGLU),
+                                       (2113, 4032, 200, EPI_SWIGLU), (301, 1349, 640, EPI_F32), (40, 1349, 640, EPI_BF16)])
+@pytest.mark.parametrize("afmt", [FP8, FP4])
+def test_gemm_cut_tiles_with_aligned_rows(lib, ws, M, N, K, epi, afmt):
+    """Rows and columns that end inside a tile, output rows on 16 bytes: the
+    columns behind and the rows below stay as they were."""
+    p = Product(M, N, K, afmt, epi, pad=N % 8 != 0)
+    assert p.ldo % 8 == 0
+    x0 = tl.to_bf16(p.x0) if p.bf16 else p.x0
+    o = tl.Dev.of(np.concatenate([x0, np.full((300, p.ldo), 7, x0.dtype)]))
+    done(lib, lib.iris_hip_mx_gemm(ctypes.byref(p.args(o.ptr)), ws.ptr, WS))
+    got = o.get(x0.dtype, (M + 300, p.ldo))
+    p.check(got[:M])
+    assert (got[M:] == 7).all()
+    o.close()
+    p.close()
+
+
 @pytest.mark.parametrize("M,N,K", [(2113, 4032, 200), (2304, 4096, 640)])
 @pytest.mark.parametrize("afmt", [FP8, FP4])
 @pytest.mark.parametrize("mx_fmt", [None, FP8, FP4])
