@@ -380,8 +380,8 @@ int iris_hip_mx_rmsnorm(const iris_mx_norm_t *a);
  * epilogues of iris_hip_gemm: F32, BF16, GATED_ADD, ADD with vec as there, and
  * SWIGLU (N % 64 == 0, no vec) into bf16 rows, or with mx_out.q set into the
  * microscaled rows mx_out instead (out unused), from the f32 values and with
- * their padding. Any M, N, K; rows up to 2^23 bytes apart take the fast
- * kernels. d_ws (or NULL): f32 workspace, 16-byte aligned, that lets products
+ * their padding. Any M, N, K up to 2^30; rows up to 2^23 bytes apart take the
+ * fast kernels. d_ws (or NULL): f32 workspace, 16-byte aligned, that lets products
  * of few tiles be split over K, summed in a fixed order. Calls that share a
  * workspace must not overlap. f32 results are f32 sums. 16- and 8-bit results
  * with e4m3 A may come from sums that drop, in each group of 8 columns, bits of

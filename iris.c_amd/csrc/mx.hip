@@ -1339,16 +1339,28 @@ extern "C" int iris_hip_mx_rmsnorm(const iris_mx_norm_t *a) {
     P.vw = rows16(a->w, 0, 4);
     P.vs = rows16(a->scale, 0, 4);
     const int dt = !a->d ? 0 : a->d_bf16 ? 2 : 1;
-    if (a->out.fmt == IRIS_MX_FP8) {
-        if (dt == 0) launch_norm<IRIS_MX_FP8, 0>(P, a->rows);
-        else if (dt == 1) launch_norm<IRIS_MX_FP8, 1>(P, a->rows);
-        else launch_norm<IRIS_MX_FP8, 2>(P, a->rows);
-    } else {
-        if (dt == 0) launch_norm<IRIS_MX_FP4, 0>(P, a->rows);
-        else if (dt == 1) launch_norm<IRIS_MX_FP4, 1>(P, a->rows);
-        else launch_norm<IRIS_MX_FP4, 2>(P, a->rows);
+    const int most = 1 << 22;   /* rows of 512 threads in one launch, which takes 2^32 threads */
+    for (int r0 = 0, nr; r0 < a->rows; r0 += nr) {
+        nr = a->rows - r0 < most ? a->rows - r0 : most;
+        if (a->out.fmt == IRIS_MX_FP8) {
+            if (dt == 0) launch_norm<IRIS_MX_FP8, 0>(P, nr);
+            else if (dt == 1) launch_norm<IRIS_MX_FP8, 1>(P, nr);
+            else launch_norm<IRIS_MX_FP8, 2>(P, nr);
+        } else {
+            if (dt == 0) launch_norm<IRIS_MX_FP4, 0>(P, nr);
+            else if (dt == 1) launch_norm<IRIS_MX_FP4, 1>(P, nr);
+            else launch_norm<IRIS_MX_FP4, 2>(P, nr);
+        }
+        if (iris_launch_check("mx_rmsnorm_kernel")) return -1;
+        P.x += (size_t)nr * P.ldx;
+        if (dt) {
+            P.d = (const char *)P.d + (size_t)nr * P.ldd * (dt == 2 ? 2 : 4);
+            P.x_out += (size_t)nr * P.ldxo;
+        }
+        P.q += (size_t)nr * P.ld_q;
+        P.s += (size_t)nr * P.ld_s;
     }
-    return iris_launch_check("mx_rmsnorm_kernel");
+    return 0;
 }
 
 /* ---- which kernel, and whether K is split ---- */
@@ -1532,7 +1544,8 @@ int mx_run(const iris_mx_gemm_t *p, float *ws, size_t ws_bytes) {
     }
     P.tiles_m = plan.tiles_m; P.tiles_n = plan.tiles_n; P.chunks = plan.chunks; P.per_chunk = plan.per_chunk;
     const long long blocks = (long long)plan.tiles_m * plan.tiles_n * plan.chunks;
-    if (blocks > 0x7fffffff / 2) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
+    /* a launch takes 2^32 threads */
+    if (blocks > 0xffffffffLL / 1024) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
     MxGemm R = P;
     if (plan.chunks > 1) {
         P.out = ws; P.ldo = p->N; P.vec = nullptr; P.epi = IRIS_EPI_F32; P.oq = nullptr;
@@ -1569,6 +1582,7 @@ extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_by
     if (!p) return iris_set_error("mx_gemm: null problem");
     if (p->M <= 0 || p->N <= 0) return 0;
     if (p->K <= 0) return iris_set_error("mx_gemm: K %d", p->K);
+    if (p->M > (1 << 30) || p->N > (1 << 30)) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
     if (check_mx("mx_gemm A", p->A, p->K) || check_mx("mx_gemm W", p->W, p->K)) return -1;
     if (p->W.fmt != IRIS_MX_FP4) return iris_set_error("mx_gemm: weights of format %d, not IRIS_MX_FP4", p->W.fmt);
     const bool swiglu = p->epi == IRIS_EPI_SWIGLU, mx = swiglu && p->mx_out.q;

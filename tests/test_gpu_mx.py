@@ -201,6 +201,28 @@ def test_rmsnorm(lib, rows, cols, fmt, add):
             v.close()
 
 
+def test_rmsnorm_of_millions_of_rows(lib):
+    """More rows than one launch holds threads for."""
+    rows, cols = (1 << 22) + 5, 3
+    rng = np.random.default_rng(11)
+    x, d = rng.standard_normal((rows, cols), np.float32), rng.standard_normal((rows, cols), np.float32)
+    w = np.array([1.0, 2.0, -0.5], np.float32)
+    dx, dd, dw, do = tl.Dev.of(x), tl.Dev.of(d), tl.Dev.of(w), tl.Dev(x.nbytes)
+    m = Mat(FP4, rows, cols)
+    a = mx.MxNorm(dx.ptr, cols, dd.ptr, cols, 0, None, do.ptr, cols, dw.ptr, None, m.c, rows, cols, 1e-6)
+    done(lib, lib.iris_hip_mx_rmsnorm(ctypes.byref(a)))
+    assert np.array_equal(do.get(np.float32, (rows, cols)), x + d)
+    pick = np.r_[0:7, rows // 2:rows // 2 + 7, rows - 12:rows]
+    _, y = norm_reference(x[pick], d[pick], None, w, None, 1e-6)
+    code, s = mx.quantize(y, FP4)
+    q, sc = m.get()
+    assert np.array_equal(q[pick, 0] & 15, code[:, 0]) and np.array_equal(q[pick, 0] >> 4, code[:, 1])
+    assert np.array_equal(q[pick, 1], code[:, 2]) and not q[pick, 2:64].any()
+    assert np.array_equal(sc[pick, 0], s[:, 0])
+    for v in (dx, dd, dw, do, m):
+        v.close()
+
+
 def test_rmsnorm_of_nan(lib):
     """A NaN in a row makes that row NaN and no other."""
     x = np.ones((3, 300), np.float32)

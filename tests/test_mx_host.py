@@ -92,6 +92,9 @@ def test_refusals(lib):
                dict(epi=-1), dict(epi=3, N=96), dict(epi=3, vec=P), dict(epi=3, ldo=31), dict(mx_out=mat(mx.FP8, 64)),
                dict(epi=3, N=32)):
         assert gemm(**kw) < 0, kw
+    # sizes that would pass 32 bits within a kernel
+    for kw in (dict(M=(1 << 30) + 1), dict(M=2 ** 31 - 1), dict(N=2 ** 31 - 1, ldo=2 ** 31 - 1)):
+        assert gemm(**kw) < 0 and b"output" in lib.iris_hip_last_error(), kw
     assert lib.iris_hip_mx_gemm(None, None, 0) < 0
 
 
