@@ -272,7 +272,7 @@ def _calls(s):
     if c["kind"] == "norm":
         add, cols = c["add"] != "none", c["cols"]
         return _MxNorm(s["x"].data_ptr(), cols, s["d"].data_ptr() if add else None, cols, int(c["add"] == "bf16"),
-                       s["gate"].data_ptr() if c["gate"] else None, s["x_out"].data_ptr() if add else None, cols,
+                       s["gate"].data_ptr() if add and c["gate"] else None, s["x_out"].data_ptr() if add else None, cols,
                        s["w"].data_ptr(), None, _mx(s["q"], s["s"], c["fmt"]), c["rows"], cols, EPS)
     mx = c["epi"] == "swiglu_mx"
     return _MxGemm(_mx(s["aq"], s["as"], c["afmt"]), _mx(s["wq"], s["ws"], FP4), None if mx else s["out"].data_ptr(),
