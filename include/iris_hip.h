@@ -383,10 +383,8 @@ int iris_hip_mx_rmsnorm(const iris_mx_norm_t *a);
  * their padding. Any M, N, K up to 2^30; rows up to 2^23 bytes apart take the
  * fast kernels. d_ws (or NULL): f32 workspace, 16-byte aligned, that lets products
  * of few tiles be split over K, summed in a fixed order. Calls that share a
- * workspace must not overlap. f32 results are f32 sums. 16- and 8-bit results
- * with e4m3 A may come from sums that drop, in each group of 8 columns, bits of
- * a product below 2^-13 of the largest one's power of two: 2e-5 of the result
- * in the mean square, where bf16 rounds by 2e-3. */
+ * workspace must not overlap. Every result comes from f32 sums, whatever its
+ * type and the number of rows; their order depends on both. */
 typedef struct {
     iris_mx_t A, W;
     void *out;

@@ -318,11 +318,14 @@ template <int AF> __device__ __forceinline__ void mx_chunk(MxGemm &P, int c) {
 /* The instruction adds its products in groups of 8 neighbouring columns and
  * keeps, of a group, bits down to 2^-13 of the largest product's power of two
  * (measured; between groups and with the accumulator it keeps f32). Products
- * of two e2m1 codes span 2^6 and lose nothing; those with e4m3 codes span more,
- * which leaves sums 2e-5 off (512 x 2560 x 9728). So A's e4m3 codes go through
- * it twice, those of magnitude 2 and more (exponents 1 .. 8) and those below
- * (lowest bit 2^-9 to 2^0): with W's lowest bit 2^-1 and highest 2^2 either
- * span is within 13 powers of two, and the sums are f32 sums. */
+ * of two e2m1 codes span 2^6 and lose nothing; those with e4m3 codes span more:
+ * one pass leaves sums of ordinary rows 2e-5 off (512 x 2560 x 9728), and one
+ * large product among small ones takes these away altogether. So A's e4m3 codes
+ * go through it twice, in every kernel and for every output type, those of
+ * magnitude 2 and more (exponents 1 .. 8) and those below (lowest bit 2^-9 to
+ * 2^0): with W's lowest bit 2^-1 and highest 2^2 either span is within 13 powers
+ * of two, and the sums are f32 sums. One pass took 254 us of 4608 x 20480 x 3840,
+ * two take 470 to 490. */
 template <int AF>
 __device__ __forceinline__ f32x4 mx_mfma(const u32x4 &w, const i32x8 &a, const f32x4 &c, int sw, int sa) {
     const i32x8 w8 = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
@@ -831,20 +834,21 @@ __global__ __launch_bounds__(NT) void mx_reduce_kernel(const MxGemm P, const flo
  * are, then a lane transposes the 4 x 4 bytes of a row so that the bytes of
  * lane group g (block g of each 128 columns) make one word; a fragment's lane
  * reads its word once per 512 columns and shifts it by a byte per 128.
- * Measured on 256 x 256 tiles: e4m3 A, 4608 x 20480 x 3840 with SwiGLU 263 us,
- * 2.75 PFLOP/s: 2620 cycles per K step, of which the matrix instructions are
- * 2110, at 1.8 to 2.1 GHz, the clock that such a kernel is given. e2m1 A, 4352
- * x 3840 x 10240 86.6 us, 3.95 PFLOP/s: 3310 cycles per 256 columns, the
- * instructions 2050; reading a step's fragments beside the loads into LDS takes
- * 1500 of a phase's 1650. 128 x 128 tiles, f32 sums: 512 x 2560 x 9728 in 3
- * ranges 33.0 us and their sum; A's two parts double the instructions. 4 waves
- * of 128 x 128 each read a third less from LDS, but have to issue the loads
- * between their own matrix instructions and wait for the address path there:
- * 126 to 130 us on 4096 x 4096 x 15360 e2m1 on either, 2580 cycles per e4m3
- * step (2200 if nothing were loaded), and 60 for 44 us where tiles are cut. */
+ * Measured on 256 x 256 tiles: e4m3 A, 4608 x 20480 x 3840 with SwiGLU 470 to
+ * 490 us, 1.5 PFLOP/s: bound by the matrix instructions of A's two parts, 4220
+ * cycles per K step, at the clock that such a kernel is given (128 x 128 tiles
+ * 518 to 534). e2m1 A, 4352 x 3840 x 10240 86.6 us, 3.95 PFLOP/s: 3310 cycles
+ * per 256 columns, the instructions 2050; reading a step's fragments beside the
+ * loads into LDS takes 1500 of a phase's 1650. 128 x 128 tiles, e4m3 A, f32:
+ * 512 x 2560 x 9728 in 3 ranges 33.0 us and their sum. 4 waves of 128 x 128 each
+ * read a third less from LDS, but have to issue the loads between their own
+ * matrix instructions and wait for the address path there: 126 to 130 us on
+ * 4096 x 4096 x 15360 e2m1 on either, and 60 for 44 us where tiles are cut.
+ * F32: f32 rows of an e4m3 A, without the code of the other outputs (96
+ * registers for 101). */
 __device__ __forceinline__ bool rows16_ok(const void *p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0; }
 
-template <int AF, bool SPLIT, int BM, int BN>
+template <int AF, bool F32, int BM, int BN>
 __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(MxGemm P) {
     constexpr bool F8 = AF == IRIS_MX_FP8;
     constexpr int KS = F8 ? 1 : 2, PER = 4 / KS;   /* 128 columns per step, steps per 512 columns */
@@ -966,16 +970,14 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
             for (int i = 0; i < FM; i++) {
                 const u32x4 x = a[0][i], y = a[1][i];
                 const i32x8 x8 = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-                const i32x8 hi = SPLIT ? mx_part<true>(x8) : x8;
+                const i32x8 hi = mx_part<true>(x8);
 #pragma unroll
                 for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma<AF>(w[0][j], hi, acc[i][j], sw[j], sa[i]);
-                if constexpr (SPLIT) {
-                    __builtin_amdgcn_sched_barrier(0);   /* one part in registers at a time */
-                    const i32x8 lo = mx_part<false>(x8);
+                __builtin_amdgcn_sched_barrier(0);   /* one part in registers at a time */
+                const i32x8 lo = mx_part<false>(x8);
 #pragma unroll
-                    for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma<AF>(w[0][j], lo, acc[i][j], sw[j], sa[i]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+                for (int j = 0; j < FN; j++) acc[i][j] = mx_mfma<AF>(w[0][j], lo, acc[i][j], sw[j], sa[i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         } else {
 #pragma unroll
@@ -1117,7 +1119,7 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
      * 42.7 us rather than 35.5. */
     uint8_t *const st = lds + wave * 8192;
     static_assert(sizeof(lds) >= 8 * 8192, "a wave's part");
-    if (P.epi == IRIS_EPI_BF16 && rows16_ok(P.out, P.ldo)) {
+    if (!F32 && P.epi == IRIS_EPI_BF16 && rows16_ok(P.out, P.ldo)) {
         __syncthreads();   /* every wave is done with the stages */
 #pragma unroll
         for (int ip = 0; ip < FM; ip += 2) {
@@ -1156,7 +1158,7 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
         }
         return;
     }
-    if (P.epi == IRIS_EPI_SWIGLU && !P.oq && rows16_ok(P.out, P.ldo)) {
+    if (!F32 && P.epi == IRIS_EPI_SWIGLU && !P.oq && rows16_ok(P.out, P.ldo)) {
         __syncthreads();
 #pragma unroll
         for (int ip = 0; ip < FM; ip += 2) {
@@ -1187,7 +1189,7 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
         return;
     }
     const bool aligned = (P.ldo & 3) == 0 && ((uintptr_t)P.out & 15) == 0;
-    if (P.epi == IRIS_EPI_SWIGLU) {
+    if (!F32 && P.epi == IRIS_EPI_SWIGLU) {
 #pragma unroll
         for (int i = 0; i < FM; i++)
 #pragma unroll
@@ -1412,16 +1414,17 @@ template <int AF> int launch_rows(const MxGemm &P, const MxPlan &plan, unsigned 
 }
 
 /* The kernel, the tile and the number of K ranges of least estimated time (us),
- * fitted to 130 products of 20 to 1500 rows (within 1.5 % of the fastest
- * measured choice on average, 25 % at most). A launch with its first loads and
- * last stores is 6; a round of 256 x 256 tiles 3 and per K step 0.85 (e2m1 A),
- * 1.25 (e4m3) or 2.85 (e4m3, f32 sums); one of 128 x 128 tiles 2 and 0.32,
- * 0.41 or 0.72: for f32 sums never slower, as the instructions bound both. A
- * split's partial sums and their second launch are 3 and their bytes at 4 TB/s.
- * Measured, us: 300 x 19456 x 2560 e4m3 to bf16: 24.1 on 128 x 128 tiles, 31.6
- * on 256 x 256; 512 rows 32.7 and 28.7; 512 x 2560 x 9728 to f32: 63 unsplit,
- * 36.6 in 3 ranges; 64 x 6144 x 2560: 10.7 through mx_gemm_rows_kernel, 15.1
- * on tiles; 64 x 19456 x 2560: 22.1 and 15.5. */
+ * over 190 products of 20 to 4608 rows 2 % slower than the fastest measured
+ * choice on average, 13 of them by more than 10 % (64 to 130 rows x 19456 x 2560
+ * through mx_gemm_rows_kernel, up to 26 % with e4m3 A and 47 % with e2m1). A
+ * launch with its first loads and last stores is 6; a round of 256 x 256 tiles 3
+ * and per K step 0.85 (e2m1 A) or 2.5 (e4m3); one of 128 x 128 tiles 2 and 0.32
+ * or 0.72. f32 rows of an e4m3 A take the small tiles, which were never slower
+ * for them. A split's partial sums and their second launch are 3 and their bytes
+ * at 4 TB/s. Measured, us, e4m3 A to bf16: 300 x 19456 x 2560 35.2 on 128 x 128
+ * tiles, 56.9 on 256 x 256; 1500 rows 133 and 122; 512 x 2560 x 9728 63.1
+ * unsplit, 36.2 in 3 ranges; 64 x 6144 x 2560 11.1 through mx_gemm_rows_kernel,
+ * 16.1 on tiles in 3 ranges. */
 template <int AF> void rows_waves(int fm, int *one, int *two) {
     switch (fm) {
     case 1: *one = RowsShape<AF, 1, 4>::WAVES; *two = RowsShape<AF, 1, 4>::WAVES2; break;
@@ -1431,9 +1434,8 @@ template <int AF> void rows_waves(int fm, int *one, int *two) {
     }
 }
 
-bool mx_exact(const iris_mx_gemm_t &p) {
-    /* 16- and 8-bit results are rounded 100 times coarser than what the single
-     * instruction loses; f32 results get f32 sums */
+/* f32 rows of an e4m3 A: on 128 x 128 tiles only */
+bool mx_f32_rows(const iris_mx_gemm_t &p) {
     return p.A.fmt == IRIS_MX_FP8 && p.epi != IRIS_EPI_SWIGLU && p.epi != IRIS_EPI_BF16;
 }
 
@@ -1463,7 +1465,7 @@ MxPlan mx_plan(const iris_mx_gemm_t &p, int steps, size_t ws_bytes, double *esti
             double us;
             if (kind == MX_TILE128 || kind == MX_TILE256) {
                 const bool big = kind == MX_TILE256;
-                const double step = !f8 ? (big ? 0.85 : 0.32) : mx_exact(p) ? 0.72 : big ? 1.25 : 0.41;
+                const double step = f8 ? (big ? 2.5 : 0.72) : big ? 0.85 : 0.32;
                 us = 6 + ceil(blocks / cus) * ((big ? 3 : 2) + step * q.per_chunk);
             } else if (kind == MX_ROWS) {
                 int one, two;
@@ -1490,7 +1492,7 @@ MxPlan mx_plan(const iris_mx_gemm_t &p, int steps, size_t ws_bytes, double *esti
         if (p.M <= 256) consider(MX_ROWS, fm, 4, 16 * fm, 64);
         if (p.M > 16) {
             consider(MX_TILE128, 0, 0, 128, 128);
-            if (!mx_exact(p)) consider(MX_TILE256, 0, 0, 256, 256);
+            if (!mx_f32_rows(p)) consider(MX_TILE256, 0, 0, 256, 256);
         }
     }
     *estimate = least;
@@ -1505,7 +1507,7 @@ int mx_main_rows(const iris_mx_gemm_t &p, int steps, size_t ws_bytes, double who
     const int cus = iris_cu_count() > 0 ? iris_cu_count() : 1;
     const int tm = (p.M + 255) / 256, tn = (p.N + 255) / 256;
     const long long rounds = (long long)tm * tn / cus;
-    if (mx_exact(p) || rounds < 1 || rounds * cus < tn) return 0;
+    if (mx_f32_rows(p) || rounds < 1 || rounds * cus < tn) return 0;
     const int rows = (int)(rounds * cus / tn) * 256;
     if (rows >= p.M) return 0;
     iris_mx_gemm_t part = p;
@@ -1554,7 +1556,6 @@ int mx_run(const iris_mx_gemm_t *p, float *ws, size_t ws_bytes) {
     if (plan.kind <= MX_DIRECT) {
         if (f8 ? launch_rows<IRIS_MX_FP8>(P, plan, (unsigned)blocks) : launch_rows<IRIS_MX_FP4>(P, plan, (unsigned)blocks)) return -1;
     } else {
-        const bool exact = mx_exact(*p);
         const dim3 grid((unsigned)((blocks + 7) / 8 * 8));
 #define MX_T(F, X, T) IRIS_LAUNCH((mx_gemm_tile_kernel<F, X, T, T>), grid, dim3(512), 0, iris_stream(), P)
         if (plan.kind == MX_TILE256) {
@@ -1562,7 +1563,7 @@ int mx_run(const iris_mx_gemm_t *p, float *ws, size_t ws_bytes) {
             else MX_T(IRIS_MX_FP8, false, 256);
         } else {
             if (!f8) MX_T(IRIS_MX_FP4, false, 128);
-            else if (exact) MX_T(IRIS_MX_FP8, true, 128);
+            else if (P.epi != IRIS_EPI_BF16 && P.epi != IRIS_EPI_SWIGLU) MX_T(IRIS_MX_FP8, true, 128);
             else MX_T(IRIS_MX_FP8, false, 128);
         }
 #undef MX_T

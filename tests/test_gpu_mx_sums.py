@@ -1,0 +1,153 @@
+"""Products of microscaled rows are sums in f32, whatever the output's type, the
+number of rows and the kernel.
+
+The matrix instruction drops, of 8 neighbouring columns, product bits below
+2^-13 of the largest one's power of two. The operands here have groups of 8
+columns with one product of 1024 to 1280 among products down to 2^-10, and the
+large ones cancel: a kernel that loses those bits is off by much of the result.
+
+Every product is a multiple of 2^-10 and the sum of their magnitudes is below
+2^14, so any order of adding them in f32 is exact: 24 bits. Results differ from
+64 bits by an epilogue's roundings and the output type's only."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import iris_testlib as tl
+import mx_reference as mx
+from mx_reference import FP4, FP8, Mat
+from test_gpu_mx import (EPI_ADD, EPI_BF16, EPI_F32, EPI_GATED_ADD, EPI_SWIGLU, U, WS, Product, done, kernels)
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return mx.bind(tl.hip())
+
+
+@pytest.fixture(scope="module")
+def ws():
+    return tl.Dev(WS)
+
+
+def spread_operands(M, N, K, seed=0):
+    """e4m3 rows with cancelling large values in up to 5 blocks, up to 0.25 beside them, small ones elsewhere."""
+    rng = np.random.default_rng(M + 3 * N + 7 * K + seed)
+
+    def values(top, rows, cols):
+        return rng.choice(mx.E4M3[mx.E4M3 <= top], (rows, cols)) * rng.choice([-1.0, 1.0], (rows, cols))
+    a = values(2.0 ** -6, M, K)
+    w = rng.choice(mx.E2M1, (N, K)) * rng.choice([-1.0, 1.0], (N, K))
+    blocks = K // 32
+    for b in rng.choice(blocks, min(blocks, 5), replace=False) * 32:
+        c1, c2 = b + rng.integers(8), b + 16 + rng.integers(8)
+        top = rng.choice([256.0, 288.0, 320.0], M) * rng.choice([-1.0, 1.0], M)
+        a[:, b:b + 8], a[:, b + 16:b + 24] = values(0.25, M, 8), values(0.25, M, 8)
+        a[:, c1], a[:, c2] = top, -top
+        w[:, c1] = w[:, c2] = 4.0 * rng.choice([-1.0, 1.0], N)
+    return a, w
+
+
+class Spread(Product):
+    """The same calls and checks on these operands; sums are exact."""
+
+    def __init__(self, M, N, K, epi, mx_fmt=None):
+        a, w = spread_operands(M, N, K)
+        self.A, self.W = Mat.of(a, FP8), Mat.of(w, FP4)
+        assert np.array_equal(self.A.values, a) and np.array_equal(self.W.values, w)
+        rng = np.random.default_rng(1)
+        self.M, self.N, self.K, self.epi, self.mx_fmt = M, N, K, epi, mx_fmt
+        self.nout = self.ldo = N // 2 if epi == EPI_SWIGLU else N
+        self.vec, self.dvec, self.use_vec = np.zeros(N, np.float32), tl.Dev(4 * N), False
+        self.x0 = (rng.integers(-64, 65, (M, self.ldo)) / 16.0).astype(np.float32)
+        self.bf16 = epi in (EPI_BF16, EPI_SWIGLU)
+        self.ab, self.y = np.zeros((M, N)), a @ w.T
+
+
+def test_one_pass_would_show():
+    """The operands tell f32 sums from those of one pass through the instruction, by far."""
+    a, w = spread_operands(16, 32, 640)
+    assert (np.abs(a) @ np.abs(w).T).max() < 2.0 ** 14 and not (a * 512 % 1).any()
+    p = (a[:, None, :] * w[None, :, :]).reshape(16, 32, -1, 8)
+    _, e = np.frexp(np.abs(p).max(3, keepdims=True))
+    step = np.exp2(e - 1.0 - 13)
+    once = (np.trunc(p / step) * step).sum((2, 3))
+    y = a @ w.T
+    assert tl.rel_l2(once, y) > 0.1
+    # the two parts lose nothing
+    big = np.abs(a) >= 2
+    both = 0.0
+    for part in (np.where(big, a, 0.0), np.where(big, 0.0, a)):
+        q = (part[:, None, :] * w[None, :, :]).reshape(16, 32, -1, 8)
+        _, e = np.frexp(np.abs(q).max(3, keepdims=True))
+        step = np.exp2(e - 1.0 - 13)
+        both = both + (np.trunc(q / step) * step).sum((2, 3))
+    assert np.array_equal(both, y)
+
+
+SUMS = [(7, 130, 640, "direct_kernel"), (40, 320, 2560, "rows_kernel"), (64, 320, 9000, "mx_reduce_kernel"),
+        (300, 1344, 640, "tile_kernel"), (512, 640, 9728, "mx_reduce_kernel")]
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K,want", SUMS)
+@pytest.mark.parametrize("epi", [EPI_F32, EPI_BF16, EPI_GATED_ADD, EPI_ADD])
+def test_sums(lib, ws, M, N, K, want, epi):
+    p = Spread(M, N, K, epi)
+    got = []
+    names = kernels(lib, lambda: got.append(p.run(lib, ws.ptr)))
+    assert want in " ".join(k for k, _ in names), names
+    y = p.exact()[0]
+    assert np.array_equal(got[0], tl.to_bf16(y.astype(np.float32)).reshape(M, N) if p.bf16 else y.astype(np.float32))
+    p.close()
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K,want", [(40, 320, 2560, "rows_kernel"), (37, 320, 9728, "mx_reduce_kernel"),
+                                        (300, 1344, 640, "tile_kernel"), (512, 640, 9728, "mx_reduce_kernel")])
+@pytest.mark.parametrize("mx_fmt", [None, FP8, FP4])
+def test_swiglu_sums(lib, ws, M, N, K, want, mx_fmt):
+    p = Spread(M, N, K, EPI_SWIGLU, mx_fmt)
+    names = kernels(lib, lambda: p.check(p.run(lib, ws.ptr)))
+    assert want in " ".join(k for k, _ in names), names
+    p.close()
+
+
+@gpu
+@pytest.mark.parametrize("epi,mx_fmt", [(EPI_BF16, None), (EPI_SWIGLU, None), (EPI_SWIGLU, FP8)])
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 512), (4400, 4160, 2048)])
+def test_large_tile_sums(lib, ws, M, N, K, epi, mx_fmt):
+    p = Spread(M, N, K, epi, mx_fmt)
+    names = kernels(lib, lambda: p.check(p.run(lib, ws.ptr)))
+    assert "256, 256>" in " ".join(k for k, _ in names), names
+    p.close()
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(40, 320, 2560), (300, 1344, 2560), (512, 640, 9728)])
+def test_sums_in_the_mean_square(lib, ws, M, N, K):
+    """Ordinary operands: K additions of 2^-24 of the sum each, in no common
+    direction, are off by at most sqrt(K) 2^-24 of it in the mean square (one
+    pass: 2e-5)."""
+    p = Product(M, N, K, FP8, EPI_F32)
+    p.use_vec = False
+    assert tl.rel_l2(p.run(lib, ws.ptr), p.y) < np.sqrt(K) * U
+    p.close()
+
+
+@gpu
+def test_rows_do_not_depend_on_their_number(lib, ws):
+    """A row's bf16 result among 8, 40, 300 and 4096 rows: sums exact in f32 give the same bits."""
+    M, N, K = 4096, 4096, 512
+    p = Spread(M, N, K, EPI_BF16)
+    whole = p.run(lib, ws.ptr)
+    for m in (8, 40, 300):
+        o = tl.Dev(m * N * 2)
+        g = p.args(o.ptr)
+        g.M = m
+        done(lib, lib.iris_hip_mx_gemm(ctypes.byref(g), ws.ptr, WS))
+        assert np.array_equal(o.get(np.uint16, (m, N)), whole[:m])
+        o.close()
+    p.close()
