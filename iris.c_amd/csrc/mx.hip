@@ -387,13 +387,15 @@ __device__ __forceinline__ void mx_store4(const MxGemm &P, int m, int n, const f
     }
 }
 
+/* The same in every kernel. The hardware's exponential and reciprocal would be
+ * |x| units of 2^-24 off, and 0 below -87, where 1 + exp(-x) has no normal
+ * reciprocal and the result still has 16 bits; they save 20 us of 4608 x 20480
+ * x 3840. */
+__device__ __forceinline__ float mx_silu(float x) { return x / (1.0f + expf(-x)); }
+
 /* a 64-column gate / up group from n on (gate tiles 0, 1, up tiles 2, 3): 8
  * values of row m in each of 4 lanes 16 apart, one block of 32 columns of the
- * output. Whole waves call it: the block's maximum is taken over the lanes.
- * FAST: the hardware's exponential and reciprocal, a few units of 2^-24 off, in
- * results of 16 or 8 bits; on tiles, where the correctly rounded ones took 21 us
- * of 283 (4608 x 20480 x 3840 into e4m3 rows). */
-template <bool FAST>
+ * output. Whole waves call it: the block's maximum is taken over the lanes. */
 __device__ __forceinline__ void mx_store_swiglu(const MxGemm &P, int m, int n, const f32x4 &g0, const f32x4 &g1,
                                                 const f32x4 &u0, const f32x4 &u1, bool aligned) {
     const int lg = (threadIdx.x >> 4) & 3, col = n / 2 + 4 * lg;
@@ -401,8 +403,8 @@ __device__ __forceinline__ void mx_store_swiglu(const MxGemm &P, int m, int n, c
     float y[8];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        y[r] = (FAST ? silu_fast(g0[r]) : g0[r] / (1.0f + expf(-g0[r]))) * u0[r];
-        y[4 + r] = (FAST ? silu_fast(g1[r]) : g1[r] / (1.0f + expf(-g1[r]))) * u1[r];
+        y[r] = mx_silu(g0[r]) * u0[r];
+        y[4 + r] = mx_silu(g1[r]) * u1[r];
     }
     if (!P.oq) {
         if (!in) return;
@@ -652,7 +654,7 @@ __global__ __launch_bounds__((64 * RowsShape<AF, FM, FN>::WAVES)) void mx_gemm_r
     if constexpr (FN == 4) {
         if (P.epi == IRIS_EPI_SWIGLU) {
             for (int i = wave; i < FM; i += waves)
-                mx_store_swiglu<false>(P, m0 + 16 * i + lr, n0, sum(i, 0), sum(i, 1), sum(i, 2), sum(i, 3), aligned);
+                mx_store_swiglu(P, m0 + 16 * i + lr, n0, sum(i, 0), sum(i, 1), sum(i, 2), sum(i, 3), aligned);
             return;
         }
     }
@@ -748,7 +750,7 @@ template <int AF, int FM, int FN> __global__ __launch_bounds__(512) void mx_gemm
     if constexpr (FN == 4) {
         if (P.epi == IRIS_EPI_SWIGLU) {
             for (int i = wave; i < FM; i += waves)
-                mx_store_swiglu<false>(P, m0 + 16 * i + lr, n0, sum(i, 0), sum(i, 1), sum(i, 2), sum(i, 3), aligned);
+                mx_store_swiglu(P, m0 + 16 * i + lr, n0, sum(i, 0), sum(i, 1), sum(i, 2), sum(i, 3), aligned);
             return;
         }
     }
@@ -798,7 +800,7 @@ __global__ __launch_bounds__(NT) void mx_reduce_kernel(const MxGemm P, const flo
     if (c < P.N / 2) {
         const Row8 g = sum8((c >> 5) * 64 + (c & 31)), u = sum8((c >> 5) * 64 + 32 + (c & 31));
 #pragma unroll
-        for (int j = 0; j < 8; j++) y.v[j] = g.v[j] / (1.0f + expf(-g.v[j])) * u.v[j];
+        for (int j = 0; j < 8; j++) y.v[j] = mx_silu(g.v[j]) * u.v[j];
     } else {
 #pragma unroll
         for (int j = 0; j < 8; j++) y.v[j] = 0.0f;   /* a microscaled row's padding */
@@ -1171,7 +1173,7 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
                         const f32x4 g = acc[ip + i][4 * j + h], u = acc[ip + i][4 * j + 2 + h];
                         uint16_t y[4];
 #pragma unroll
-                        for (int r = 0; r < 4; r++) y[r] = f2bf_hw(silu_fast(g[r]) * u[r]);
+                        for (int r = 0; r < 4; r++) y[r] = f2bf_hw(mx_silu(g[r]) * u[r]);
                         const int row = i * 16 + lr;
                         *(uint2 *)(st + row * TWN + (((4 * j + 2 * h + (lg >> 1)) ^ (row & (FN - 1))) << 4) + (lg & 1) * 8) =
                             make_uint2((uint32_t)y[0] | (uint32_t)y[1] << 16, (uint32_t)y[2] | (uint32_t)y[3] << 16);
@@ -1194,7 +1196,7 @@ __global__ __launch_bounds__(512, BM == 128 ? 4 : 2) void mx_gemm_tile_kernel(Mx
         for (int i = 0; i < FM; i++)
 #pragma unroll
             for (int j = 0; j < FN; j += 4)
-                mx_store_swiglu<true>(P, m0 + wm * TWM + i * 16 + lr, n0 + wn * TWN + j * 16, acc[i][j], acc[i][j + 1],
+                mx_store_swiglu(P, m0 + wm * TWM + i * 16 + lr, n0 + wn * TWN + j * 16, acc[i][j], acc[i][j + 1],
                                 acc[i][j + 2], acc[i][j + 3], aligned);
         return;
     }

@@ -151,3 +151,41 @@ def test_rows_do_not_depend_on_their_number(lib, ws):
         assert np.array_equal(o.get(np.uint16, (m, N)), whole[:m])
         o.close()
     p.close()
+
+
+class Gates(Product):
+    """SwiGLU of gates over the e4m3 range from -88 on, one gate a row (none of
+    them 0: the check takes a block's scale for that of its maximum), and an up of 2^20."""
+
+    def __init__(self, M, N, mx_fmt=None):
+        K, top = 512, mx.E4M3[(mx.E4M3 > 0) & (mx.E4M3 <= 88)]
+        top = top[np.frexp(top)[0] != 15 / 16]      # alone in a block 1.875 2^e has no code
+        a, w = np.zeros((M, K)), np.zeros((N, K))
+        a[:, 0], a[:, 32] = np.resize(np.r_[-top[::-1], top], M), 2.0 ** 20
+        gate = np.arange(N) % 64 < 32
+        w[gate, 0], w[~gate, 32] = 1.0, 1.0
+        self.A, self.W = Mat.of(a, FP8), Mat.of(w, FP4)
+        assert np.array_equal(self.A.values, a) and np.array_equal(self.W.values, w)
+        self.M, self.N, self.K, self.epi, self.mx_fmt = M, N, K, EPI_SWIGLU, mx_fmt
+        self.nout = self.ldo = N // 2
+        self.dvec, self.use_vec, self.bf16 = tl.Dev(4), False, True
+        self.x0 = np.zeros((M, self.nout), np.float32)
+        self.ab, self.y = np.zeros((M, N)), a @ w.T
+
+
+@gpu
+@pytest.mark.parametrize("mx_fmt", [None, FP8, FP4])
+def test_gates_of_every_size(lib, ws, mx_fmt):
+    """On tiles of both sizes and through the few-row kernel: against 64 bits,
+    and a row's bits whatever the number of rows."""
+    rows = {}
+    for M, N, want in ((16, 1344, "rows_kernel"), (300, 1344, "128, 128>"), (4096, 4096, "256, 256>")):
+        p = Gates(M, N, mx_fmt)
+        got = []
+        names = kernels(lib, lambda: got.append(p.run(lib, ws.ptr)))
+        assert want in " ".join(k for k, _ in names), names
+        p.check(got[0])
+        rows[M] = (got[0] if mx_fmt is None else got[0].read()[0])[:16, :672]
+        assert (np.abs(p.exact()[0]) > 1e-32).all()
+        p.close()
+    assert np.array_equal(rows[16], rows[300]) and np.array_equal(rows[16], rows[4096])
