@@ -40,6 +40,7 @@ struct qwen3_model {
     int (*mx_layer)(qwen3_model_t *m, const qlayer_t *l, const float *next_ln1, int S, int n_real);
     void (*mx_free)(qwen3_model_t *m);
     iris_mx_t a_mx, attn_mx, mlp_mx;
+    float *d_mx;                  /* [S][h], what a product adds to the stream */
 };
 
 /* Q, K, V rows of a layer (m->qkv) to its attention output (m->attn) */

@@ -37,14 +37,16 @@ static void free_all(qwen3_model_t *m) {
         release(&l->qkv_mx); release(&l->o_mx); release(&l->gate_up_mx); release(&l->down_mx);
     }
     release(&m->a_mx); release(&m->attn_mx); release(&m->mlp_mx);
+    iris_hip_free(m->d_mx);
+    m->d_mx = NULL;
 }
 
 /* residual stream += d (NULL: as it is), then the RMSNorm of it in 8 bits */
-static int mx_rms(qwen3_model_t *m, const uint16_t *d, const float *w, int S) {
+static int mx_rms(qwen3_model_t *m, const float *d, const float *w, int S) {
     iris_mx_norm_t a;
     memset(&a, 0, sizeof(a));
     a.x = a.x_out = m->x; a.ldx = a.ldxo = m->hidden;
-    a.d = d; a.ldd = m->hidden; a.d_bf16 = 1;
+    a.d = d; a.ldd = m->hidden;
     a.w = w; a.out = m->a_mx; a.rows = S; a.cols = m->hidden; a.eps = QWEN3_RMS_NORM_EPS;
     if (!d) a.x_out = NULL;
     return iris_hip_mx_rmsnorm(&a);
@@ -61,23 +63,23 @@ static int mx_gemm(qwen3_model_t *m, const iris_mx_t *A, const iris_mx_t *W, voi
 
 static int first(qwen3_model_t *m, int S) { return mx_rms(m, NULL, m->L[0].ln1, S); }
 
-/* a layer, from its normalised input rows to those of the next layer: the residual's additions run in the
- * norms that read the stream next; the last layer's, which no norm follows, in
- * its product */
+/* a layer, from its normalised input rows to those of the next layer: the
+ * residual's additions, of f32 sums as in the bf16 layer, run in the norms that
+ * read the stream next; the last layer's, which no norm follows, in its product */
 static int layer(qwen3_model_t *m, const qlayer_t *l, const float *next_ln1, int S, int n_real) {
     const int h = m->hidden, qd = m->heads * HD, kd = m->kv_heads * HD, I = m->inter;
     CK(mx_gemm(m, &m->a_mx, &l->qkv_mx, m->qkv, qd + 2 * kd, S, qd + 2 * kd, h, IRIS_EPI_BF16, NULL));
     if (iris_qwen3_attend(m, l, S, n_real)) return -1;
     CK(iris_hip_mx_quantize(&m->attn_mx, m->attn, 1, qd, S, qd));
-    CK(mx_gemm(m, &m->attn_mx, &l->o_mx, m->a, h, S, h, qd, IRIS_EPI_BF16, NULL));
-    CK(mx_rms(m, m->a, l->ln2, S));
+    CK(mx_gemm(m, &m->attn_mx, &l->o_mx, m->d_mx, h, S, h, qd, IRIS_EPI_F32, NULL));
+    CK(mx_rms(m, m->d_mx, l->ln2, S));
     CK(mx_gemm(m, &m->a_mx, &l->gate_up_mx, NULL, 0, S, 2 * I, h, IRIS_EPI_SWIGLU, &m->mlp_mx));
     if (!next_ln1) {
         CK(mx_gemm(m, &m->mlp_mx, &l->down_mx, m->x, h, S, h, I, IRIS_EPI_GATED_ADD, NULL));
         return 0;
     }
-    CK(mx_gemm(m, &m->mlp_mx, &l->down_mx, m->a, h, S, h, I, IRIS_EPI_BF16, NULL));
-    CK(mx_rms(m, m->a, next_ln1, S));
+    CK(mx_gemm(m, &m->mlp_mx, &l->down_mx, m->d_mx, h, S, h, I, IRIS_EPI_F32, NULL));
+    CK(mx_rms(m, m->d_mx, next_ln1, S));
     return 0;
 }
 
@@ -86,7 +88,7 @@ int qwen3_model_quantize(qwen3_model_t *m) {
     if (m->mx_layer) return 0;
     const int h = m->hidden, I = m->inter, qd = m->heads * HD, kd = m->kv_heads * HD, S = QWEN3_MAX_SEQ_LEN;
     int rc = room(&m->a_mx, IRIS_MX_FP8, S, h) || room(&m->attn_mx, IRIS_MX_FP8, S, qd) ||
-             room(&m->mlp_mx, IRIS_MX_FP8, S, I);
+             room(&m->mlp_mx, IRIS_MX_FP8, S, I) || !(m->d_mx = (float *)iris_hip_malloc((size_t)S * h * sizeof(float)));
     for (int i = 0; !rc && i < m->layers; i++) {
         qlayer_t *l = &m->L[i];
         rc = room(&l->qkv_mx, IRIS_MX_FP4, (size_t)qd + 2 * kd, h) || room(&l->o_mx, IRIS_MX_FP4, h, qd) ||
