@@ -461,11 +461,14 @@ constexpr int GROUP_M = 8;
  * stage the compiler waits for the builtin's loads into the others too, which
  * takes the ring's depth away. The caller waits (vmcnt) before a barrier. */
 __device__ __forceinline__ uint32_t lds_at(const void *p) { return (uint32_t)(uintptr_t)(const lds_void *)p; }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   /* m0 is reserved: the compiler keeps nothing in it, but may write it for its own use */
 __device__ __forceinline__ void load_lds16(const u32x4 &rsrc, uint32_t at, int voff, int soff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  ::"s"(at), "v"(voff), "s"(rsrc), "s"(soff)
-                 : "memory");
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ u32x4 buffer_of(const void *p, int bytes) {
     const uint64_t a = (uint64_t)(uintptr_t)p;
     return (u32x4){(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)),
