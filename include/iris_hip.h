@@ -380,11 +380,13 @@ int iris_hip_mx_rmsnorm(const iris_mx_norm_t *a);
  * epilogues of iris_hip_gemm: F32, BF16, GATED_ADD, ADD with vec as there, and
  * SWIGLU (N % 64 == 0, no vec) into bf16 rows, or with mx_out.q set into the
  * microscaled rows mx_out instead (out unused), from the f32 values and with
- * their padding. Any M, N, K up to 2^30; rows up to 2^23 bytes apart take the
- * fast kernels. d_ws (or NULL): f32 workspace, 16-byte aligned, that lets products
- * of few tiles be split over K, summed in a fixed order. Calls that share a
- * workspace must not overlap. Every result comes from f32 sums, whatever its
- * type and the number of rows; their order depends on both. */
+ * their padding. Any M, N, K up to 2^30 whose launch takes fewer than 2^32
+ * threads, others are refused (one row by 2^27 columns of K 4096; f32 results of
+ * 2^30 rows by 128); rows less than 2^23 bytes apart take the fast kernels.
+ * d_ws (or NULL): f32 workspace, 16-byte aligned, that lets products of few tiles
+ * be split over K, summed in a fixed order. Calls that share a workspace must not
+ * overlap. Every result comes from f32 sums, whatever its type and the number of
+ * rows; their order depends on both. */
 typedef struct {
     iris_mx_t A, W;
     void *out;

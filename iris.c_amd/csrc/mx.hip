@@ -1377,13 +1377,24 @@ struct MxPlan {
     int kind, fm, fn, tiles_m, tiles_n, chunks, per_chunk;
 };
 
-template <int AF, int FM, int FN> int launch_rows_of(const MxGemm &P, unsigned blocks) {
-    using Sh = RowsShape<AF, FM, FN>;
-    /* units of 256 columns, as evenly as the waves that LDS holds take them */
-    /* two blocks on a CU where there are more than CUs: 37 x 19456 x 2560, 304
-     * blocks, 17.0 us, 21.8 with one block of all waves */
-    const int most = (int)blocks <= iris_cu_count() ? Sh::WAVES : Sh::WAVES2;
-    const int units = (P.per_chunk + 1) / 2;
+/* waves that LDS holds of mx_gemm_rows_kernel, one block per CU and two */
+template <int AF> void rows_waves(int fm, int *one, int *two) {
+    switch (fm) {
+    case 1: *one = RowsShape<AF, 1, 4>::WAVES; *two = RowsShape<AF, 1, 4>::WAVES2; break;
+    case 2: *one = RowsShape<AF, 2, 4>::WAVES; *two = RowsShape<AF, 2, 4>::WAVES2; break;
+    case 3: *one = RowsShape<AF, 3, 4>::WAVES; *two = RowsShape<AF, 3, 4>::WAVES2; break;
+    default: *one = RowsShape<AF, 4, 4>::WAVES; *two = RowsShape<AF, 4, 4>::WAVES2; break;
+    }
+}
+
+/* waves of a block: units of 256 columns, as evenly as those that LDS holds take
+ * them; two blocks on a CU where there are more than CUs (37 x 19456 x 2560, 304
+ * blocks: 17.0 us, 21.8 with one block of all waves) */
+template <int AF> int rows_block_waves(int fm, int per_chunk, long long blocks) {
+    int one, two;
+    rows_waves<AF>(fm, &one, &two);
+    const int most = blocks <= iris_cu_count() ? one : two;
+    const int units = (per_chunk + 1) / 2;
     /* rounds of a unit per wave: its loads, about two units' instructions, and
      * the instructions of the SIMD with the most waves */
     int waves = 1;
@@ -1392,6 +1403,16 @@ template <int AF, int FM, int FN> int launch_rows_of(const MxGemm &P, unsigned b
         const int cost = 2 * (full + (rest > 0)) + full * ((w + 3) / 4) + (rest + 3) / 4;
         if (cost < least) least = cost, waves = w;
     }
+    return waves;
+}
+/* and of mx_gemm_direct_kernel: a wave per 512 columns, as evenly as 8 waves take them */
+int direct_block_waves(int per_chunk) {
+    const int groups = (per_chunk + 3) / 4, rounds = (groups + 7) / 8;
+    return (groups + rounds - 1) / rounds;
+}
+
+template <int AF, int FM, int FN> int launch_rows_of(const MxGemm &P, unsigned blocks, int waves) {
+    using Sh = RowsShape<AF, FM, FN>;
     const int smem = Sh::SCALES + waves * Sh::UNIT;
     static_assert(Sh::UNIT >= FM * FN * 1024, "the sums fit where the units were");
     static std::once_flag once;
@@ -1404,18 +1425,16 @@ template <int AF, int FM, int FN> int launch_rows_of(const MxGemm &P, unsigned b
     IRIS_LAUNCH((mx_gemm_rows_kernel<AF, FM, FN>), dim3(blocks), dim3(64 * waves), smem, iris_stream(), P);
     return 0;
 }
-template <int AF> int launch_rows(const MxGemm &P, const MxPlan &plan, unsigned blocks) {
+template <int AF> int launch_rows(const MxGemm &P, const MxPlan &plan, unsigned blocks, int waves) {
     if (plan.kind == MX_DIRECT) {
-        /* a wave per 512 columns, as evenly as 8 waves take them */
-        const int groups = (P.per_chunk + 3) / 4, rounds = (groups + 7) / 8, waves = (groups + rounds - 1) / rounds;
         if (plan.fn == 1) IRIS_LAUNCH((mx_gemm_direct_kernel<AF, 1, 1>), dim3(blocks), dim3(64 * waves), waves * 1024, iris_stream(), P);
         else IRIS_LAUNCH((mx_gemm_direct_kernel<AF, 1, 4>), dim3(blocks), dim3(64 * waves), waves * 4096, iris_stream(), P);
         return 0;
     }
-    if (plan.fm == 1) return launch_rows_of<AF, 1, 4>(P, blocks);
-    if (plan.fm == 2) return launch_rows_of<AF, 2, 4>(P, blocks);
-    if (plan.fm == 3) return launch_rows_of<AF, 3, 4>(P, blocks);
-    return launch_rows_of<AF, 4, 4>(P, blocks);
+    if (plan.fm == 1) return launch_rows_of<AF, 1, 4>(P, blocks, waves);
+    if (plan.fm == 2) return launch_rows_of<AF, 2, 4>(P, blocks, waves);
+    if (plan.fm == 3) return launch_rows_of<AF, 3, 4>(P, blocks, waves);
+    return launch_rows_of<AF, 4, 4>(P, blocks, waves);
 }
 
 /* The kernel, the tile and the number of K ranges of least estimated time (us),
@@ -1430,15 +1449,6 @@ template <int AF> int launch_rows(const MxGemm &P, const MxPlan &plan, unsigned 
  * tiles, 56.9 on 256 x 256; 1500 rows 133 and 122; 512 x 2560 x 9728 63.1
  * unsplit, 36.2 in 3 ranges; 64 x 6144 x 2560 11.1 through mx_gemm_rows_kernel,
  * 16.1 on tiles in 3 ranges. */
-template <int AF> void rows_waves(int fm, int *one, int *two) {
-    switch (fm) {
-    case 1: *one = RowsShape<AF, 1, 4>::WAVES; *two = RowsShape<AF, 1, 4>::WAVES2; break;
-    case 2: *one = RowsShape<AF, 2, 4>::WAVES; *two = RowsShape<AF, 2, 4>::WAVES2; break;
-    case 3: *one = RowsShape<AF, 3, 4>::WAVES; *two = RowsShape<AF, 3, 4>::WAVES2; break;
-    default: *one = RowsShape<AF, 4, 4>::WAVES; *two = RowsShape<AF, 4, 4>::WAVES2; break;
-    }
-}
-
 /* f32 rows of an e4m3 A: on 128 x 128 tiles only */
 bool mx_f32_rows(const iris_mx_gemm_t &p) {
     return p.A.fmt == IRIS_MX_FP8 && p.epi != IRIS_EPI_SWIGLU && p.epi != IRIS_EPI_BF16;
@@ -1550,18 +1560,26 @@ int mx_run(const iris_mx_gemm_t *p, float *ws, size_t ws_bytes) {
         return mx_run(&part, ws, ws_bytes);
     }
     P.tiles_m = plan.tiles_m; P.tiles_n = plan.tiles_n; P.chunks = plan.chunks; P.per_chunk = plan.per_chunk;
-    const long long blocks = (long long)plan.tiles_m * plan.tiles_n * plan.chunks;
-    /* a launch takes 2^32 threads */
-    if (blocks > 0xffffffffLL / 1024) return iris_set_error("mx_gemm: %d x %d output", p->M, p->N);
+    const bool f8 = p->A.fmt == IRIS_MX_FP8;
+    long long blocks = (long long)plan.tiles_m * plan.tiles_n * plan.chunks;
+    if (plan.kind > MX_DIRECT) blocks = (blocks + 7) / 8 * 8;   /* as many for each XCD */
+    const int waves = plan.kind > MX_DIRECT ? 8
+                    : plan.kind == MX_DIRECT ? direct_block_waves(plan.per_chunk)
+                    : f8 ? rows_block_waves<IRIS_MX_FP8>(plan.fm, plan.per_chunk, blocks)
+                         : rows_block_waves<IRIS_MX_FP4>(plan.fm, plan.per_chunk, blocks);
+    if (blocks * 64 * waves > 0xffffffffLL)
+        return iris_set_error("mx_gemm: %d x %d output of K %d, more than 2^32 threads", p->M, p->N, p->K);
+    if (!iris_hip_available()) return -1;
     MxGemm R = P;
     if (plan.chunks > 1) {
         P.out = ws; P.ldo = p->N; P.vec = nullptr; P.epi = IRIS_EPI_F32; P.oq = nullptr;
     }
-    const bool f8 = p->A.fmt == IRIS_MX_FP8;
     if (plan.kind <= MX_DIRECT) {
-        if (f8 ? launch_rows<IRIS_MX_FP8>(P, plan, (unsigned)blocks) : launch_rows<IRIS_MX_FP4>(P, plan, (unsigned)blocks)) return -1;
+        if (f8 ? launch_rows<IRIS_MX_FP8>(P, plan, (unsigned)blocks, waves)
+               : launch_rows<IRIS_MX_FP4>(P, plan, (unsigned)blocks, waves))
+            return -1;
     } else {
-        const dim3 grid((unsigned)((blocks + 7) / 8 * 8));
+        const dim3 grid((unsigned)blocks);
 #define MX_T(F, X, T) IRIS_LAUNCH((mx_gemm_tile_kernel<F, X, T, T>), grid, dim3(512), 0, iris_stream(), P)
         if (plan.kind == MX_TILE256) {
             if (!f8) MX_T(IRIS_MX_FP4, false, 256);
@@ -1600,6 +1618,6 @@ extern "C" int iris_hip_mx_gemm(const iris_mx_gemm_t *p, float *ws, size_t ws_by
     const int nout = swiglu ? p->N / 2 : p->N;
     if (mx ? check_mx("mx_gemm output", p->mx_out, nout) : !p->out ? iris_set_error("mx_gemm: null output") : 0) return -1;
     if (!mx && p->ldo < nout) return iris_set_error("mx_gemm: output row stride %d of %d columns", p->ldo, nout);
-    if (!iris_hip_available()) return -1;
+    (void)iris_hip_available();   /* the plan counts the device's CUs; sizes are refused without one, too */
     return mx_run(p, ws, ((uintptr_t)ws & 15) || !ws ? 0 : ws_bytes);
 }
