@@ -362,8 +362,8 @@ int iris_hip_mx_dequantize(void *d_y, int is_bf16, int ldy, const iris_mx_t *a, 
  *   out = t / sqrt(mean(t^2) + eps) * w (* scale if given), microscaled
  * t goes to x_out (required with d, not written without it): x itself with its
  * row stride, or rows that overlap neither x nor d. The statistics are held in
- * 64 bits and the codes are those of the exact quotient of t's f32 values. x,
- * d, x_out of any alignment. */
+ * 64 bits and the codes are those of the exact quotient of t's f32 values, one
+ * past the range of f32 as its largest number. x, d, x_out of any alignment. */
 typedef struct {
     const float *x; int ldx;
     const void *d; int ldd; int d_bf16;   /* f32 rows, or bf16 */
