@@ -335,7 +335,8 @@ int iris_hip_rms_gated_add(float *d_x, const float *d_y, const float *d_w, const
  * bytes, ld_q and ld_s are multiples of 16 and at least iris_hip_mx_ld_codes
  * and iris_hip_mx_ld_scales of the columns (the scale bytes from the padded
  * columns to the next multiple of 16 are never read for their value). Rows of
- * a checkpoint in this format are used as they are. */
+ * a checkpoint in this format are used as they are where they hold whole 512
+ * columns; others need this padding. */
 enum { IRIS_MX_FP8 = 0, IRIS_MX_FP4 = 1 };
 typedef struct {
     uint8_t *q, *s;      /* codes, scales */

@@ -217,8 +217,8 @@ template <int DT> __device__ __forceinline__ Row8 norm_row8(const NormParams &P,
     return x;
 }
 
-/* Bound by the bytes, one pass over them: 4608 x 3840, bf16 d and gate, 42.5 us
- * (4.6 TB/s); 512 x 2560, f32 d, 5.7 us; one row 4.6 us, a launch.
+/* Bound by the bytes, one pass over them: 4608 x 3840, bf16 d and gate, 41.0 us
+ * (4.8 TB/s); 512 x 2560, f32 d, 4.7 us; one row 3.5 us, a launch.
  * DT: 0 no d, 1 f32, 2 bf16. One block of TH threads per row, R chunks of 8
  * columns a thread held in registers; R 0: any length, the row read twice (the second
  * time from x_out where there is a d: the thread's own stores). */
@@ -324,8 +324,8 @@ template <int AF> __device__ __forceinline__ void mx_chunk(MxGemm &P, int c) {
  * go through it twice, in every kernel and for every output type, those of
  * magnitude 2 and more (exponents 1 .. 8) and those below (lowest bit 2^-9 to
  * 2^0): with W's lowest bit 2^-1 and highest 2^2 either span is within 13 powers
- * of two, and the sums are f32 sums. One pass took 254 us of 4608 x 20480 x 3840,
- * two take 470 to 490. */
+ * of two, and the sums are f32 sums. 4608 x 20480 x 3840 with SwiGLU takes 490 to
+ * 505 us so, 254 with one pass. */
 template <int AF>
 __device__ __forceinline__ f32x4 mx_mfma(const u32x4 &w, const i32x8 &a, const f32x4 &c, int sw, int sa) {
     const i32x8 w8 = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
@@ -389,8 +389,8 @@ __device__ __forceinline__ void mx_store4(const MxGemm &P, int m, int n, const f
 
 /* The same in every kernel. The hardware's exponential and reciprocal would be
  * |x| units of 2^-24 off, and 0 below -87, where 1 + exp(-x) has no normal
- * reciprocal and the result still has 16 bits; they save 20 us of 4608 x 20480
- * x 3840. */
+ * reciprocal and the result still has 16 bits; they would save 20 to 25 of 490 us
+ * of 4608 x 20480 x 3840. */
 __device__ __forceinline__ float mx_silu(float x) { return x / (1.0f + expf(-x)); }
 
 /* a 64-column gate / up group from n on (gate tiles 0, 1, up tiles 2, 3): 8
@@ -521,10 +521,12 @@ __device__ __forceinline__ f32x4 mx_sum_waves(const f32x4 *part, int stride, int
  * each line twice, and a wave's loads in registers leave room for half the
  * waves: gate and up of 37 rows 24.8 us. Scales of 4096 columns are loaded by
  * the whole block, a line a row. The waves' sums are added in wave order.
- * Measured, e4m3 A: 37 x 19456 x 2560 with SwiGLU 14.3 us (26.5 MB of W at 1.9
+ * Measured, e4m3 A: 37 x 19456 x 2560 with SwiGLU 14.7 us (26.5 MB of W at 1.8
  * TB/s; of a block's 10 us a third is launch, first loads and scales, a third
  * instructions, a third sums and epilogue), 37 x 6144 x 2560 8.6; e2m1 A: 37 x
- * 11520 x 3840 7.3 (3.2 TB/s). */
+ * 11520 x 3840 7.3 (3.2 TB/s). <e2m1, 4, 4> spills 7 registers, addresses of the
+ * next unit's loads, and waits for the loads in flight at each reload: 256 x 3840
+ * x 10240 22.7 us. */
 template <int AF, int FM, int FN> struct RowsShape {
     static constexpr int A_ROW = AF == IRIS_MX_FP8 ? 256 : 128;    /* bytes of 256 columns */
     static constexpr int A_BYTES = FM * 16 * A_ROW, UNIT = A_BYTES + FN * 2048;
@@ -839,18 +841,21 @@ __global__ __launch_bounds__(NT) void mx_reduce_kernel(const MxGemm P, const flo
  * are, then a lane transposes the 4 x 4 bytes of a row so that the bytes of
  * lane group g (block g of each 128 columns) make one word; a fragment's lane
  * reads its word once per 512 columns and shifts it by a byte per 128.
- * Measured on 256 x 256 tiles: e4m3 A, 4608 x 20480 x 3840 with SwiGLU 470 to
- * 490 us, 1.5 PFLOP/s: bound by the matrix instructions of A's two parts, 4220
- * cycles per K step, at the clock that such a kernel is given (128 x 128 tiles
- * 518 to 534). e2m1 A, 4352 x 3840 x 10240 86.6 us, 3.95 PFLOP/s: 3310 cycles
- * per 256 columns, the instructions 2050; reading a step's fragments beside the
- * loads into LDS takes 1500 of a phase's 1650. 128 x 128 tiles, e4m3 A, f32:
- * 512 x 2560 x 9728 in 3 ranges 33.0 us and their sum. 4 waves of 128 x 128 each
- * read a third less from LDS, but have to issue the loads between their own
- * matrix instructions and wait for the address path there: 126 to 130 us on
- * 4096 x 4096 x 15360 e2m1 on either, and 60 for 44 us where tiles are cut.
- * F32: f32 rows of an e4m3 A, without the code of the other outputs (96
- * registers for 101). */
+ * Measured on 256 x 256 tiles: e4m3 A, 4608 x 20480 x 3840 with SwiGLU 490 to
+ * 505 us, 1.45 PFLOP/s: bound by the matrix instructions of A's two parts, 4220
+ * cycles per K step, at the clock that such a kernel is given (with the
+ * hardware's SwiGLU 482, on 128 x 128 tiles 534). It spills one sum in one of
+ * four steps of group 1 (24 bytes a lane); the compiler's wait for the reload also
+ * waits for the loads in flight. e2m1 A, 4352 x 3840 x 10240 86.6 us, 3.95
+ * PFLOP/s: 3310 cycles per 256 columns, the instructions 2050; reading a step's
+ * fragments beside the loads into LDS takes 1500 of a phase's 1650. 128 x 128
+ * tiles, e4m3 A, f32: 512 x 2560 x 9728 in 3 ranges 33 us and their sum. 4 waves
+ * of 128 x 128 each read a third less from LDS, but have to issue the loads
+ * between their own matrix instructions and wait for the address path there: 126
+ * to 130 us on 4096 x 4096 x 15360 e2m1 on either, and 60 for 44 us where tiles
+ * are cut.
+ * F32: f32 rows of an e4m3 A, without the code of the other outputs: 96 registers
+ * for 101, 512 x 6144 x 2560 24.6 us for 24.9. */
 __device__ __forceinline__ bool rows16_ok(const void *p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0; }
 
 template <int AF, bool F32, int BM, int BN>
