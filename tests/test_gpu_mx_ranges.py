@@ -1,5 +1,6 @@
-"""Microscaled operators where a call is cut: products with SwiGLU split over K,
-more rows than one launch takes, quotients past the range of f32."""
+"""Microscaled operators where a call is cut: products split over K, SwiGLU behind
+them, captured ones, more rows than one launch takes, quotients past the range of
+f32."""
 import ctypes
 
 import numpy as np
@@ -8,7 +9,7 @@ import pytest
 import iris_testlib as tl
 import mx_reference as mx
 from mx_reference import FP4, FP8, Mat
-from test_gpu_mx import EPI_SWIGLU, WS, Product, done, kernels
+from test_gpu_mx import EPI_BF16, EPI_F32, EPI_GATED_ADD, EPI_SWIGLU, WS, Product, done, kernels
 
 pytestmark = pytest.mark.gpu
 
@@ -44,6 +45,61 @@ def test_swiglu_of_split_products(lib, ws, M, N, K, afmt, mx_fmt):
         assert (q[:, mx.ld_codes(mx_fmt, p.nout):] == 0xA5).all() and (s[:, mx.ld_scales(p.nout):] == 0xA5).all()
         m.close()
     p.close()
+
+
+@pytest.mark.parametrize("M,N,K,want", [(3, 70, 100000, "direct_kernel"), (40, 64, 100000, "rows_kernel"),
+                                        (300, 192, 30000, "tile_kernel")])
+@pytest.mark.parametrize("afmt", [FP8, FP4])
+@pytest.mark.parametrize("epi", [EPI_F32, EPI_GATED_ADD])
+def test_long_sums(lib, ws, M, N, K, want, afmt, epi):
+    """Ten times the longest row of a model, in ranges and in one; a range that ends inside a step."""
+    p = Product(M, N, K, afmt, epi)
+    names = " ".join(k for k, _ in kernels(lib, lambda: p.check(p.run(lib, ws.ptr))))
+    assert want in names and "mx_reduce_kernel" in names, names
+    p.check(p.run(lib, None, 0))
+    p.close()
+
+
+@pytest.mark.parametrize("M,N,K,epi,mx_fmt,launches", [(37, 320, 9728, EPI_SWIGLU, FP8, 2), (64, 320, 9000, EPI_GATED_ADD, None, 2),
+                                                       (4400, 4160, 2000, EPI_BF16, None, 2)])
+def test_captured(lib, ws, M, N, K, epi, mx_fmt, launches):
+    """A product of several launches in a graph, replayed with eager products
+    that use the same workspace between: the eager bits each time."""
+    p = Product(M, N, K, FP8, epi, mx_fmt=mx_fmt)
+    x0 = tl.to_bf16(p.x0) if p.bf16 else p.x0
+    m = Mat(mx_fmt, M, p.nout) if mx_fmt is not None else None
+    o = None if m else tl.Dev.of(x0)
+    g = p.args(o.ptr if o else None, m)
+
+    def put():
+        if m:
+            m.q.put(np.full(m.shape_q, 0xA5, np.uint8))
+            m.s.put(np.full(m.shape_s, 0xA5, np.uint8))
+        else:
+            o.put(x0)
+
+    def get():
+        assert lib.iris_hip_sync() == 0
+        return m.get() if m else (o.get(x0.dtype, x0.shape),)
+    names = kernels(lib, lambda: done(lib, lib.iris_hip_mx_gemm(ctypes.byref(g), ws.ptr, WS)))
+    assert sum(("mx_" in k) for k, _ in names) >= launches, names
+    want = get()
+    lib.iris_hip_graph_end.restype = ctypes.c_void_p
+    lib.iris_hip_graph_launch.argtypes = lib.iris_hip_graph_destroy.argtypes = [ctypes.c_void_p]
+    assert lib.iris_hip_graph_begin() == 0
+    rc = lib.iris_hip_mx_gemm(ctypes.byref(g), ws.ptr, WS)
+    graph = lib.iris_hip_graph_end()
+    assert rc == 0 and graph
+    e = Product(64, 320, 9000, FP8, EPI_F32)
+    for _ in range(4):
+        put()
+        e.check(e.run(lib, ws.ptr))
+        assert lib.iris_hip_graph_launch(graph) == 0
+        for a, b in zip(get(), want):
+            assert np.array_equal(a, b)
+    lib.iris_hip_graph_destroy(graph)
+    for v in (p, e, m or o):
+        v.close()
 
 
 def test_quantize_of_many_rows(lib):
